@@ -457,6 +457,81 @@ int mb_attention_decode_static(mb_ctx* ctx, mb_stream stream, const void* q, con
                                size_t batch, size_t nq, size_t keys, size_t heads, size_t kv_heads, size_t d,
                                size_t q0, float scale, int causal, void* out);
 
+/* ---- paged cache with device block tables ------------------------------------------- */
+/* Serving a continuous batch: every sequence keeps its rows in pages of one shared pool, in any order, and the
+ * lengths live on the device, so that one captured graph serves every step. It continues the page lists of the
+ * reference's cache (KvPages, src/models/inkling/kvpages.rs:1378-1404; KeyRun, src/models/inkling/flash.rs:995-1015),
+ * whose runs are described on the host and shared by all sequences of a call.
+ *
+ * Pools: k, v [pages, page_size, kv_heads * d] bf16 (MB_KV_BF16), or E2M1 codes [pages, page_size, kv_heads * d / 2]
+ * with E4M3 scales [pages, page_size, kv_heads * d / 16] (MB_KV_NVFP4; blocks of 16 along the features, the bytes
+ * mb_nvfp4_quantize_act writes with MB_QUANT_RECIP for the bf16 rows). d is 64 or 128, page_size a multiple of 16.
+ * Row r of sequence b is row r % page_size of page block_table[b * table_stride + r / page_size]; lens[b] counts
+ * its rows, the tokens of the call included (append first, then attend). Both are read by the kernels only.
+ * Entries that no row in use needs (past the length, below a window) may hold anything.
+ *
+ * Bad tables are contained: a length outside [0, table_width * page_size] is clamped to it, a needed entry outside
+ * [0, pages) reads as rows of zeros and takes no append; either raises the plan flag of the context
+ * (sequence + 1, mb_check_flags). Rows at or past the length may hold anything, NaN included. */
+typedef struct mb_paged_kv {
+  void* k;
+  void* v;
+  void* k_scales;             /* MB_KV_NVFP4 only, else NULL */
+  void* v_scales;
+  int elem;                   /* MB_KV_BF16 or MB_KV_NVFP4 */
+  size_t pages, page_size, kv_heads, d;
+  const int32_t* block_table; /* [batch, table_stride], the first table_width entries of a row are its pages */
+  size_t table_width, table_stride;
+  const int32_t* lens;        /* [batch] */
+  size_t batch;
+} mb_paged_kv;
+
+/* What happens to a score s = scale * q.k of the query at position p and the key at position k:
+ * s' = softcap * tanh(s / softcap) when softcap > 0, then s' - slopes[head] * |p - k| when slopes is given
+ * ([heads] f32). The key is visible when k <= p and, with window > 0, p - k < window; keys k < prefix[b]
+ * (prefix [batch] i32 or NULL) are visible to every query of sequence b, later ones included: a two-way prefix, or,
+ * beside a window, first rows that stay in sight. A query that sees no key gets a row of zeros. */
+typedef struct mb_score_terms {
+  float scale;
+  float softcap;
+  size_t window;
+  const float* slopes;
+  const int32_t* prefix;
+} mb_score_terms;
+
+/* Rotation and append for ragged tokens: qkv [tokens, qkv_stride] bf16 holds stacked projections
+ * (hq + 2 kv_heads) * d wide. Sequence b owns tokens [cu_q[b], cu_q[b + 1]) (cu_q [batch + 1] i32, ascending from 0),
+ * or, with cu_q NULL, tokens [b * n, (b + 1) * n) with n = tokens / batch; they are its last rows. q heads are rotated
+ * into q_out [tokens, hq * d]; k heads are rotated and v heads copied (quantized in an NVFP4 pool) into the pages.
+ * Pairs are (f, f + d / 2) as in mb_rope. The angle is position * inv_freq[f] taken in 64 bits, sine and cosine are
+ * 32-bit and the rotated value is rounded once (mb_rope keeps the rounding points of its own bf16 tables). The position
+ * of a token is its row, or positions[a * tokens + token] (i32, `axes` rows of `tokens`) with the axis a of frequency f
+ * given by section_end: the first a with f < section_end[a] (axes <= 4, ascending, the last one d / 2; time, height
+ * and width of image and video tokens). Tokens at or past cu_q[batch] are left alone, their rows of q_out too. */
+int mb_paged_append(mb_ctx* ctx, mb_stream stream, const void* qkv, size_t qkv_stride, size_t tokens, size_t hq,
+                    const mb_paged_kv* kv, const int32_t* cu_q, const float* inv_freq, const int32_t* positions,
+                    size_t axes, const int32_t* section_end, void* q_out);
+
+/* Attention of the last nq tokens of every sequence: q, out [batch, nq, heads * d] bf16, query i of sequence b at
+ * position lens[b] - nq + i (a negative position gets a row of zeros). The work of the whole batch is cut evenly over
+ * the SMs whatever the lengths: a CTA takes a run of 64-row tiles that may span several sequences and heads, pieces
+ * of the same rows are joined by a second kernel in a fixed order. workspace: mb_paged_decode_workspace bytes,
+ * 256-byte aligned, no initial contents; calls that may overlap need one each. */
+size_t mb_paged_decode_workspace(mb_ctx* ctx, const mb_paged_kv* kv, size_t nq, size_t heads);
+int mb_paged_decode(mb_ctx* ctx, mb_stream stream, const void* q, size_t nq, size_t heads, const mb_paged_kv* kv,
+                    const mb_score_terms* terms, void* out, void* workspace, size_t workspace_bytes);
+
+/* The same for ragged blocks of query tokens, fresh prompts and chunks over what the cache already holds: q, out
+ * [tokens, heads * d] bf16, sequence b owns tokens [cu_q[b], cu_q[b + 1]) (i32, ascending from 0), which are its last
+ * rows; no query sees another sequence. Rows of `out` at or past cu_q[batch] are left alone. heads / kv_heads <= 128.
+ * tcgen05 tiles of 128 (token, head of the group) rows; where the tokens give fewer blocks than the device has SMs the
+ * keys are cut as well and the parts joined from `workspace` in a fixed order (mb_paged_prompt_workspace bytes, 256-byte
+ * aligned, may be 0; calls that may overlap need one each). Every sum runs over the rows some query of a block sees, so
+ * a NaN or an infinity in a live row of V reaches the other queries of that block. */
+size_t mb_paged_prompt_workspace(mb_ctx* ctx, const mb_paged_kv* kv, size_t tokens, size_t heads);
+int mb_paged_prompt(mb_ctx* ctx, mb_stream stream, const void* q, size_t tokens, size_t heads, const mb_paged_kv* kv,
+                    const int32_t* cu_q, const mb_score_terms* terms, void* out, void* workspace, size_t workspace_bytes);
+
 /* ---- decoder-layer glue (Breeze rounding points) ------------------------------------ */
 /* norm_kernel (src/models/breeze/cuda_ops.rs:88-117): bf16(bf16(x*inv)*gain). */
 int mb_rmsnorm(mb_ctx* ctx, mb_stream stream, const void* x_bf16, const void* gain_bf16, size_t rows,

@@ -31,6 +31,21 @@ class KeyRun(C.Structure):
                 ("rows", C.c_size_t), ("base", C.c_size_t), ("lo", C.c_size_t), ("hi", C.c_size_t),
                 ("row0", C.c_size_t)]
 
+
+class PagedKv(C.Structure):
+    """mb_paged_kv: a paged cache with device block tables and lengths."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scales", C.c_void_p), ("v_scales", C.c_void_p),
+                ("elem", C.c_int), ("pages", C.c_size_t), ("page_size", C.c_size_t), ("kv_heads", C.c_size_t),
+                ("d", C.c_size_t), ("block_table", C.c_void_p), ("table_width", C.c_size_t), ("table_stride", C.c_size_t),
+                ("lens", C.c_void_p), ("batch", C.c_size_t)]
+
+
+class ScoreTerms(C.Structure):
+    """mb_score_terms: scale, cap, window, distance bias and prefix of an attention call over a paged cache."""
+    _fields_ = [("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_size_t), ("slopes", C.c_void_p),
+                ("prefix", C.c_void_p)]
+
+
 _vp, _sz, _f, _i = C.c_void_p, C.c_size_t, C.c_float, C.c_int
 
 SIGNATURES = {
@@ -85,6 +100,11 @@ SIGNATURES = {
                                _sz, _f, _vp, _i, _vp, _sz]),
     "mb_attention_decode_static_warm": (_i, [_vp]),
     "mb_attention_decode_static": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _sz, _sz, _f, _i, _vp]),
+    "mb_paged_append": (_i, [_vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
+    "mb_paged_decode_workspace": (_sz, [_vp, _vp, _sz, _sz]),
+    "mb_paged_decode": (_i, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _sz]),
+    "mb_paged_prompt_workspace": (_sz, [_vp, _vp, _sz, _sz]),
+    "mb_paged_prompt": (_i, [_vp, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _sz]),
     "mb_rmsnorm": (_i, [_vp, _vp, _vp, _vp, _sz, _sz, _f, _vp]),
     "mb_rmsnorm_inkling": (_i, [_vp, _vp, _vp, _i, _vp, _sz, _sz, _f, _vp, _i]),
     "mb_gate_up_silu": (_i, [_vp, _vp, _vp, _i, _sz, _sz, _i, _vp, _i]),

@@ -56,6 +56,7 @@ struct mb_ctx {
   std::mutex scratch_mu;
   // which one-time set-up steps this context has done (a context belongs to one device)
   std::atomic<uint32_t> once{0};
+  std::atomic<uint32_t> paged_once{0};   // the same for the variants of the paged-cache kernels
   int pair_clusters = 0;             // CTA pairs of the pair GEMM the device holds at once (0 = not asked yet)
   // clusters of 2..8 CTAs of the single-CTA GEMM kernels (split-K through distributed shared memory) the device
   // holds at once, per kernel variant (NVFP4 / bf16 x column width): 0 = not asked yet, -1 = none

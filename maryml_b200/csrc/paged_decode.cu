@@ -1,0 +1,751 @@
+// Attention of the last few tokens of every sequence over a paged cache (head_dim 64 or 128, bf16 or NVFP4 rows).
+//
+// The mathematics is the one-pass softmax: over the key tiles of a query row, m = running reference, l = sum 2^(s - m),
+// o = sum 2^(s - m) v, all in f32; partial (m, l, o) of disjoint key sets join by m* = max m, l* = sum l 2^(m - m*),
+// o* likewise. The reference m only has to lie near the true maximum (P, l and o scale together), so it is moved, and o
+// rescaled, only when a score exceeds it by a wide margin: no cross-lane maximum in the common tile.
+//
+// Bound by HBM for bf16 rows (each row of a sequence is read once, all query heads of a KV head ride along) and by
+// instruction issue for NVFP4 rows (the expansion of codes).
+//
+// Split. The lengths are known to the device only and differ from sequence to sequence, so the unit of work is one
+// 64-row tile of one (sequence, KV head, row tile) item; the tiles of all items form one line that is cut evenly over
+// a grid of fixed size. A CTA's run of tiles is a list of pieces, at most the first and the last of which cover their
+// item only in part: those go to the workspace (two slots per CTA), whole items are written directly. The join kernel
+// finds an item's pieces by arithmetic and adds them in tile order, so a call gives the same bits every time.
+//
+// Layout. Keys are the M side of both products (S^T = K Q^T, O^T = V^T P^T, mma.sync m16n8k16): with up to eight query
+// rows an 8-wide N tile holds them all (16 query rows on the M side waste half the products and the accumulators),
+// and P^T becomes an operand by one 8 x 8 transpose of packed pairs. Four compute warps take 16 rows each of a tile.
+// bf16 tiles arrive by TMA through a ring of three stages (boxes of up to 64 rows that do not cross a page); NVFP4 rows
+// come as packed bytes through a cp.async ring per warp, and are expanded to f16 in registers.
+#include "paged.cuh"
+
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+namespace {
+
+using namespace tc5;
+
+constexpr int BC = 64;                  // rows per tile
+constexpr int STAGES = 3;
+constexpr uint32_t MIN_TILES = 2;       // tiles a CTA takes at least: fewer would spend more on the join than on the rows
+// How far (in powers of two) a score may exceed the reference m before m moves, and how far below the maximum m is then
+// put. Probabilities in f16 (beside four-bit rows) sit in its upper range, [2^7, 2^15] at the top, so that one of 2^-21 of
+// the largest is still a normal number; bf16 has the range of f32.
+constexpr float LAG_BF16 = 8.0f, LAG_F16 = 15.0f, DROP_F16 = 7.0f;
+
+struct DecodeParams {
+  CUtensorMap tmap_k, tmap_v;           // bf16 pools
+  PagedView c;
+  const uint8_t *k, *v, *ks, *vs;       // NVFP4 pools
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  const float* slopes;
+  uint4* meta;                          // per item: first slot, pieces, first CTA
+  float* part;                          // [2 * grid][16][D + 2]: o, m, l
+  uint32_t nq, heads, group, rows, row_tiles;   // rows = nq * group
+  uint32_t box_rows;
+  float scale, scale_log2, cap_log2, inv_cap;   // cap_log2 = softcap * log2(e), inv_cap = scale / softcap
+  int* flags;
+};
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool F16>
+__device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b) {
+  if (F16)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                 "{%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, __half2 b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Four bytes of E2M1 pairs -> four f16x2 registers (low nibble = low half), exact.
+__device__ __forceinline__ void e2m1x8_to_f16(uint32_t w, uint32_t* h) {
+  asm("{ .reg .b8 b0, b1, b2, b3; mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3; }"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3]) : "r"(w));
+}
+__device__ __forceinline__ __half2 e4m3x2_to_f16(uint32_t two_bytes) {
+  uint32_t h;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(two_bytes)));
+  return *reinterpret_cast<__half2*>(&h);
+}
+
+// Byte offset of (row, 16-byte chunk) in a tile stored as 64-feature halves of 128-byte rows under the 128-byte swizzle.
+__device__ __forceinline__ uint32_t tile_off(uint32_t row, uint32_t c) {
+  return (c >> 3) * (BC * 128) + row * 128u + (((c & 7u) ^ (row & 7u)) << 4);
+}
+
+// The line of tiles: sequence b contributes span.count() * kv_heads * row_tiles of them.
+__device__ __forceinline__ PagedSpan decode_span(const PagedView& c, uint32_t b, uint32_t nq, int& len) {
+  len = paged_len(c, b);
+  return paged_span(c, b, len, len - int(nq), len - 1, BC);
+}
+struct LinePlace {
+  unsigned long long total;       // tiles of the line
+  uint32_t per;                   // tiles of a CTA
+  uint32_t b;                     // sequence that holds the tile asked for
+  unsigned long long before;      // tiles before that sequence
+};
+// One warp: the line's length, and where tile `per * cta` of it lies.
+__device__ __forceinline__ LinePlace line_place(const PagedView& c, uint32_t nq, uint32_t items, uint32_t grid, uint32_t cta,
+                                                uint32_t lane) {
+  LinePlace at;
+  unsigned long long sum = 0;
+  int len;
+  for (uint32_t i = lane; i < c.batch; i += 32) sum += (unsigned long long)(decode_span(c, i, nq, len).count()) * items;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  at.total = sum;
+  at.per = max(MIN_TILES, uint32_t((sum + grid - 1) / grid));
+  const unsigned long long want = (unsigned long long)at.per * cta;
+  at.b = c.batch;
+  at.before = 0;
+  unsigned long long base = 0;
+  for (uint32_t i0 = 0; i0 < c.batch; i0 += 32) {
+    unsigned long long mine = i0 + lane < c.batch ? (unsigned long long)(decode_span(c, i0 + lane, nq, len).count()) * items : 0ull;
+    unsigned long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long up = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= uint32_t(o)) inc += up;
+    }
+    const uint32_t hit = __ballot_sync(0xFFFFFFFFu, base + inc > want);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      at.b = i0 + src;
+      at.before = base + __shfl_sync(0xFFFFFFFFu, inc - mine, src);
+      break;
+    }
+    base += __shfl_sync(0xFFFFFFFFu, inc, 31);
+  }
+  return at;
+}
+
+template <int D, bool FP4, int NT>
+struct DecodeShape {
+  static constexpr int THREADS = FP4 ? 128 : 160;
+  static constexpr int TILE_BYTES = BC * D * 2;                              // K or V tile, bf16
+  static constexpr int RAW_WARP = 2 * 16 * (D / 2) + 2 * 16 * (D / 16);      // a warp's packed rows of K and V
+  static constexpr int RING = FP4 ? 4 * STAGES * RAW_WARP : 2 * STAGES * TILE_BYTES;
+  static constexpr int PATCH = NT * 8 * (D + 4) * 4 + 2 * 4 * NT * 8 * 4;     // o of a piece; m and l of the four warps
+  static constexpr int SMEM = RING + PATCH + 1024 + 256;
+  static constexpr int CTAS = FP4 ? (NT == 1 ? 4 : 3) : 2;
+};
+
+template <int D, bool FP4, int NT>
+__global__ void __launch_bounds__(DecodeShape<D, FP4, NT>::THREADS, DecodeShape<D, FP4, NT>::CTAS)
+paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+  using Shape = DecodeShape<D, FP4, NT>;
+  constexpr int KS = D / 16, HALVES = D / 64, TILE = Shape::TILE_BYTES, ROWS = NT * 8, PD = D + 4;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  float* patch = reinterpret_cast<float*>(gen + Shape::RING);       // [ROWS][PD]
+  float* stat_m = patch + ROWS * PD;                                // [4][ROWS]
+  float* stat_l = stat_m + 4 * ROWS;
+  const uint32_t bar_base = base + Shape::RING + Shape::PATCH;
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+  uint32_t* place = reinterpret_cast<uint32_t*>(gen + Shape::RING + Shape::PATCH + 16 * STAGES);   // b, offset, tiles
+  volatile int* abort_smem = reinterpret_cast<volatile int*>(place + 4);
+  volatile int* gave_up = abort_smem + 1;        // set by compute warps only, between two of their barriers
+  int* tflag = p.flags ? p.flags + MB_FLAG_WAIT_TIMEOUT : nullptr;
+  const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x >> 5), 0);
+  const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3u;
+  const uint32_t items = p.c.kv_heads * p.row_tiles;
+
+  if (threadIdx.x == 0) {
+    if (!FP4) {
+      for (int s = 0; s < STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 4); }
+      fence_barrier_init();
+      tma_prefetch_desc(&p.tmap_k);
+      tma_prefetch_desc(&p.tmap_v);
+    }
+    *abort_smem = 0;
+    *gave_up = 0;
+  }
+  mb_grid_dependency_sync();
+  if (warp == 0) {
+    const LinePlace at = line_place(p.c, p.nq, items, gridDim.x, blockIdx.x, lane);
+    if (lane == 0) {
+      const unsigned long long first = (unsigned long long)at.per * blockIdx.x;
+      place[0] = at.b;
+      place[1] = uint32_t(first - at.before);
+      place[2] = first < at.total ? uint32_t(min((unsigned long long)at.per, at.total - first)) : 0u;
+      place[3] = at.per;
+    }
+  }
+  __syncthreads();
+  uint32_t left = place[2];
+  if (left == 0) return;
+  const uint32_t per = place[3];
+  uint32_t b = place[0], skip = place[1];        // tiles of sequence b that lie before this CTA's first
+
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true, first_piece = true;
+  while (left > 0 && b < p.c.batch) {
+    int len;
+    const PagedSpan span = decode_span(p.c, b, p.nq, len);
+    const uint32_t n = span.count();
+    if (n == 0 || skip >= n * items) { skip = n ? skip - n * items : skip; ++b; continue; }
+    const uint32_t item = skip / n, i0 = skip - item * n, cnt = min(left, n - i0);
+    const uint32_t kvh = item / p.row_tiles, r_first = (item - kvh * p.row_tiles) * 16u;
+    const int q_first = len - int(p.nq);
+
+    if (!FP4 && warp == 4) {
+      // ------------------------------ producer: tiles by TMA ------------------------------
+      const uint32_t per_tile = BC / p.box_rows;
+      // the next 32 boxes' pages, a lane each, fetched a window ahead
+      auto pages_of = [&](uint32_t box) -> uint32_t {
+        const uint32_t i = i0 + box / per_tile;
+        if (i >= i0 + cnt) return p.c.pages;
+        const uint32_t r = span.tile_down(i) * BC + (box % per_tile) * p.box_rows;
+        if (!span.needed(int(r), int(p.box_rows))) return p.c.pages;       // zeros: nothing there is seen
+        return paged_page(p.c, b, mb_fastdiv_q(r, p.c.page_div));
+      };
+      uint32_t ids = pages_of(lane), ids_next = pages_of(lane + 32);
+      for (uint32_t i = 0; i < cnt; ++i) {
+        if (!mbar_wait(empty_bar(stage), phase ^ 1u, abort_smem, tflag, 11)) { ok = false; break; }
+        const uint32_t box0 = (i * per_tile) & 31u;
+        if (box0 == 0 && i > 0) {
+          ids = ids_next;
+          ids_next = pages_of(i * per_tile + 32 + lane);
+        }
+        const uint32_t s0 = base + stage * 2 * TILE;
+        const uint32_t row0 = span.tile_down(i0 + i) * BC;
+        if (elect_one()) mbar_arrive_expect_tx(full_bar(stage), 2 * TILE);
+        __syncwarp();
+        for (uint32_t x = 0; x < per_tile; ++x) {
+          const uint32_t page = __shfl_sync(0xFFFFFFFFu, ids, box0 + x);
+          const uint32_t r = row0 + x * p.box_rows, in_page = r - mb_fastdiv_q(r, p.c.page_div) * p.c.page_size;
+          const uint32_t dst = s0 + x * p.box_rows * 128u;
+          if (elect_one()) {
+#pragma unroll
+            for (int hf = 0; hf < HALVES; ++hf) {
+              asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                           ::"r"(dst + hf * (BC * 128)), "l"(&p.tmap_k), "r"(hf * 64), "r"(int(kvh)), "r"(int(in_page)),
+                             "r"(int(page)), "r"(full_bar(stage)) : "memory");
+              asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                           ::"r"(dst + TILE + hf * (BC * 128)), "l"(&p.tmap_v), "r"(hf * 64), "r"(int(kvh)), "r"(int(in_page)),
+                             "r"(int(page)), "r"(full_bar(stage)) : "memory");
+            }
+          }
+          __syncwarp();
+        }
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+      }
+    } else {
+      // ------------------------------ compute warps: rows 16 w .. 16 w + 15 of a tile ------------------------------
+      // Q as the B operand: query g of N tile nt, features 16 ks + 2 t4 (and + 8); with NVFP4 rows the features run in
+      // the order the packed bytes give them, 4 of lane t4's D / 4 per step (and f16: exact for magnitudes in
+      // [2^-14, 65504], larger ones saturate).
+      uint32_t qf[KS][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint32_t r = r_first + nt * 8 + g;
+        const bool live = r < p.rows;
+        const uint32_t qi = live ? r / p.group : 0u, hg = live ? r - qi * p.group : 0u;
+        const __nv_bfloat16* src = p.q + ((size_t(b) * p.nq + qi) * p.heads + kvh * p.group + hg) * D;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t d0 = FP4 ? (D / 4) * t4 + 4 * ks + 2 * e : 16 * ks + 2 * t4 + 8 * e;
+            uint32_t v = live ? __ldg(reinterpret_cast<const uint32_t*>(src + d0)) : 0u;
+            if (FP4)
+              v = pack_f16(fminf(fmaxf(__uint_as_float(v << 16), -65504.0f), 65504.0f),
+                           fminf(fmaxf(__uint_as_float(v & 0xFFFF0000u), -65504.0f), 65504.0f));
+            qf[ks][nt][e] = v;
+          }
+        }
+      }
+      // this lane's score columns: queries 2 t4 and 2 t4 + 1 of each N tile
+      int qpos[NT][2];
+      float slope[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t r = r_first + nt * 8 + 2 * t4 + e;
+          const bool live = r < p.rows;
+          const uint32_t qi = live ? r / p.group : p.nq - 1, hg = live ? r - qi * p.group : 0u;
+          qpos[nt][e] = q_first + int(qi);
+          slope[nt][e] = p.slopes ? __ldg(p.slopes + kvh * p.group + hg) * 1.4426950408889634f : 0.0f;
+        }
+      float o[KS][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) m[nt][0] = m[nt][1] = -INFINITY, l[nt][0] = l[nt][1] = 0.0f;
+
+      // NVFP4: the warp's own ring of packed rows. A tile's 16 rows lie in one page (16 divides the page size).
+      uint8_t* ring = gen + uint32_t(warp) * STAGES * Shape::RAW_WARP;
+      uint32_t ids = p.c.pages, ids_next = p.c.pages;
+      auto page_of = [&](uint32_t i) -> uint32_t {
+        if (i >= cnt) return p.c.pages;
+        const uint32_t r = span.tile_down(i0 + i) * BC + uint32_t(warp) * 16u;
+        if (!span.needed(int(r), 16)) return p.c.pages;
+        return paged_page(p.c, b, mb_fastdiv_q(r, p.c.page_div));
+      };
+      auto issue = [&](uint32_t i) {
+        if (i < cnt) {
+          if ((i & 31u) == 0 && i > 0) { ids = ids_next; ids_next = page_of(i + 32 + lane); }
+          const uint32_t page = __shfl_sync(0xFFFFFFFFu, ids, i & 31u);
+          const uint32_t r = span.tile_down(i0 + i) * BC + uint32_t(warp) * 16u;
+          const uint32_t in_page = r - mb_fastdiv_q(r, p.c.page_div) * p.c.page_size;
+          const bool have = page < p.c.pages;
+          const size_t row0 = (size_t(have ? page : 0u) * p.c.page_size + (have ? in_page : 0u)) * p.c.kv_heads + kvh;
+          const uint32_t dst = smem_u32(ring + (i % STAGES) * Shape::RAW_WARP);
+          constexpr int PER = D / 32;                   // 16-byte chunks of a row's codes
+#pragma unroll
+          for (int u = 0; u < (16 * PER) / 32; ++u) {
+            const uint32_t x = lane + 32 * u, row = x / PER;
+            const uint32_t bytes = have && int(r + row) < len ? 16u : 0u;
+            const size_t off = (row0 + size_t(bytes ? row : 0u) * p.c.kv_heads) * (D / 2) + (x % PER) * 16u;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + x * 16u), "l"(p.k + off), "r"(bytes) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 16 * (D / 2) + x * 16u), "l"(p.v + off), "r"(bytes) : "memory");
+          }
+          {
+            const uint32_t row = lane & 15u;
+            const uint32_t bytes = have && int(r + row) < len ? uint32_t(D / 16) : 0u;
+            const uint8_t* src = (lane < 16 ? p.ks : p.vs) + (row0 + size_t(bytes ? row : 0u) * p.c.kv_heads) * (D / 16);
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst + 16 * D + lane * (D / 16)), "l"(src), "r"(bytes),
+                         "n"(D / 16) : "memory");
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      if (FP4) {
+        ids = page_of(lane);
+        ids_next = page_of(32 + lane);
+#pragma unroll
+        for (uint32_t s = 0; s < STAGES; ++s) issue(s);
+      }
+
+      for (uint32_t i = 0; i < cnt; ++i) {
+        const uint32_t tile = span.tile_down(i0 + i);
+        const int row0 = int(tile * BC) + warp * 16;       // this warp's first row
+        const uint8_t* raw = ring + (i % STAGES) * Shape::RAW_WARP;
+        if (FP4) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+          __syncwarp();
+        } else if (!mbar_wait(full_bar(stage), phase, abort_smem, tflag, 12)) { ok = false; break; }
+        const uint32_t k_s = base + stage * 2 * TILE, v_s = k_s + TILE;
+
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+        if (FP4) {
+          // lane (g, t4): rows g and g + 8, features (D / 4) t4 .. of each
+          uint32_t wlo[D / 32], whi[D / 32];
+          __half2 sc[2][D / 64];                            // scales of the two rows, (D / 64) blocks each
+#pragma unroll
+          for (int x = 0; x < D / 64; ++x) {
+            const uint32_t* lo = reinterpret_cast<const uint32_t*>(raw + g * (D / 2) + t4 * (D / 8)) + 2 * x;
+            const uint32_t* hi = reinterpret_cast<const uint32_t*>(raw + (g + 8) * (D / 2) + t4 * (D / 8)) + 2 * x;
+            const uint2 a = *reinterpret_cast<const uint2*>(lo), c2 = *reinterpret_cast<const uint2*>(hi);
+            wlo[2 * x] = a.x; wlo[2 * x + 1] = a.y;
+            whi[2 * x] = c2.x; whi[2 * x + 1] = c2.y;
+            sc[0][x] = __low2half2(e4m3x2_to_f16(raw[16 * D + g * (D / 16) + t4 * (D / 64) + x]));
+            sc[1][x] = __low2half2(e4m3x2_to_f16(raw[16 * D + (g + 8) * (D / 16) + t4 * (D / 64) + x]));
+          }
+#pragma unroll
+          for (int w = 0; w < D / 32; ++w) {                // a word of codes: two K steps
+            uint32_t hl[4], hh[4];
+            e2m1x8_to_f16(wlo[w], hl);
+            e2m1x8_to_f16(whi[w], hh);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t a[4] = {hmul2(hl[2 * e], sc[0][w / 2]), hmul2(hh[2 * e], sc[1][w / 2]),
+                                     hmul2(hl[2 * e + 1], sc[0][w / 2]), hmul2(hh[2 * e + 1], sc[1][w / 2])};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma<true>(s[nt], a, qf[2 * w + e][nt]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t a[4];
+            ldsm_x4(k_s + tile_off(warp * 16 + (lane & 15u), ks * 2 + (lane >> 4)), a);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma<false>(s[nt], a, qf[ks][nt]);
+          }
+          // The stage before this one goes back to the producer now, a whole score pass after its last reads.
+          if (i > 0 || !first_piece) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty_bar(stage == 0 ? STAGES - 1 : stage - 1));
+          }
+        }
+
+        // scores in units of log2: cap, bias, mask
+        const bool whole = row0 + 16 <= span.prefix ||
+                           (row0 + 16 <= q_first + 1 && (p.c.window == 0 || row0 > len - 1 - int(p.c.window)));
+        float x[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = row0 + int(g) + (e >= 2 ? 8 : 0), qp = qpos[nt][e & 1];
+            float y = p.cap_log2 > 0.0f ? p.cap_log2 * paged_tanh(s[nt][e] * p.inv_cap) : s[nt][e] * p.scale_log2;
+            if (p.slopes) y = fmaf(-slope[nt][e & 1], fabsf(float(qp - key)), y);
+            if (!whole) {
+              const bool seen = (key < len && key <= qp && (p.c.window == 0 || qp - key < int(p.c.window))) || key < span.prefix;
+              y = seen ? y : -INFINITY;
+            }
+            x[nt][e] = y;
+          }
+        bool grown = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) grown |= x[nt][e] > m[nt][e & 1] + (FP4 ? LAG_F16 : LAG_BF16);
+        if (__any_sync(0xFFFFFFFFu, grown)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(x[nt][e], x[nt][e + 2]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 16));
+              const float m_new = fmaxf(m[nt][e], FP4 ? mx - DROP_F16 : mx);
+              const float f = m[nt][e] == -INFINITY ? 0.0f : paged_ex2(m[nt][e] - m_new);
+              m[nt][e] = m_new;
+              l[nt][e] *= f;
+#pragma unroll
+              for (int d = 0; d < KS; ++d) { o[d][nt][e] *= f; o[d][nt][e + 2] *= f; }
+            }
+        }
+        // P^T: bf16 (f16 beside four-bit rows); its rounding is what the 16-bit products take, l sums the unrounded f32
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float pr[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) pr[e] = x[nt][e] == -INFINITY ? 0.0f : paged_ex2(x[nt][e] - m[nt][e & 1]);
+          l[nt][0] += pr[0] + pr[2];
+          l[nt][1] += pr[1] + pr[3];
+          pb[nt][0] = transpose8x8(FP4 ? pack_f16(pr[0], pr[1]) : pack_bf16(pr[0], pr[1]));
+          pb[nt][1] = transpose8x8(FP4 ? pack_f16(pr[2], pr[3]) : pack_bf16(pr[2], pr[3]));
+        }
+
+        if (FP4) {
+          // lane (g, t4): features (D / 8) g .. of rows 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9. The nibbles of a row pair are
+          // interleaved first, so that one conversion gives both rows' value of a feature: tile i of O^T holds features
+          // (D / 8) g + 2 i (rows 0..7 of the tile) and + 1 (rows 8..15).
+          constexpr int W = D / 64;                       // words of codes per row
+          uint32_t w[4][W];
+          __half2 sc[2];                                  // scales of the row pairs (2 t4, 2 t4 + 1), (2 t4 + 8, 2 t4 + 9)
+          const uint8_t* vraw = raw + 16 * (D / 2);
+          const uint8_t* vsc = raw + 16 * D + 16 * (D / 16);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t row = 2u * t4 + (q & 1u) + 8u * (q >> 1);
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(vraw + row * (D / 2) + g * (D / 16));
+            if (W == 2) {
+              const uint2 a = *reinterpret_cast<const uint2*>(src);
+              w[q][0] = a.x; w[q][W - 1] = a.y;
+            } else {
+              w[q][0] = *src;
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t row = 2u * t4 + 8u * h, blk = g * (D / 8) / 16;
+            sc[h] = e4m3x2_to_f16(uint32_t(vsc[row * (D / 16) + blk]) | uint32_t(vsc[(row + 1) * (D / 16) + blk]) << 8);
+          }
+#pragma unroll
+          for (int y = 0; y < W; ++y) {
+            uint32_t ev[2][4], od[2][4];                  // even and odd features of the two row pairs
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a = w[2 * h][y], c2 = w[2 * h + 1][y];
+              e2m1x8_to_f16((a & 0x0F0F0F0Fu) | ((c2 << 4) & 0xF0F0F0F0u), ev[h]);
+              e2m1x8_to_f16(((a >> 4) & 0x0F0F0F0Fu) | (c2 & 0xF0F0F0F0u), od[h]);
+            }
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+              const uint32_t a[4] = {hmul2(ev[0][i4], sc[0]), hmul2(od[0][i4], sc[0]), hmul2(ev[1][i4], sc[1]), hmul2(od[1][i4], sc[1])};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) mma<true>(o[4 * y + i4][nt], a, pb[nt]);
+            }
+          }
+          __syncwarp();                                   // the warp is done with the ring slot
+          issue(i + STAGES);
+        } else {
+          if (!whole) {
+            // rows nobody sees may hold NaN (behind the length, below the window), and 0 * NaN is NaN: zeros instead
+            for (uint32_t x2 = lane; x2 < 16u * (D / 8); x2 += 32) {
+              const uint32_t row = x2 / (D / 8);
+              const int key = row0 + int(row);
+              if (!((key < span.k_hi && key >= span.k_lo) || key < span.prefix))
+                *reinterpret_cast<uint4*>(gen + (v_s - base) + tile_off(warp * 16 + row, x2 % (D / 8))) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async();                          // before the stage is filled by TMA again
+            __syncwarp();
+          }
+          const uint32_t mi = lane >> 3, l8 = lane & 7u;
+#pragma unroll
+          for (int d = 0; d < KS; ++d) {
+            uint32_t a[4];
+            ldsm_x4_trans(v_s + tile_off(warp * 16 + (mi >> 1) * 8 + l8, d * 2 + (mi & 1u)), a);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma<false>(o[d][nt], a, pb[nt]);
+          }
+          first_piece = false;
+          if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        }
+      }
+      if (FP4) asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+      // ---- join the four warps: m, l first, then o through the patch in warp order ----
+      if (!ok && lane == 0) *gave_up = 1;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], 4);
+          l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], 8);
+          l[nt][e] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][e], 16);
+          if (g == 0) {
+            stat_m[warp * ROWS + nt * 8 + 2 * t4 + e] = m[nt][e];
+            stat_l[warp * ROWS + nt * 8 + 2 * t4 + e] = l[nt][e];
+          }
+        }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (*gave_up) ok = false;                            // all four leave the loop together
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t r = nt * 8 + 2 * t4 + e;
+          const float mm = fmaxf(fmaxf(stat_m[r], stat_m[ROWS + r]), fmaxf(stat_m[2 * ROWS + r], stat_m[3 * ROWS + r]));
+          const float f = m[nt][e] == -INFINITY ? 0.0f : paged_ex2(m[nt][e] - mm);
+#pragma unroll
+          for (int d = 0; d < KS; ++d) { o[d][nt][e] *= f; o[d][nt][e + 2] *= f; }
+        }
+#pragma unroll 1
+      for (int w = 3; w >= 0; --w) {
+        if (warp == w) {
+#pragma unroll
+          for (int d = 0; d < KS; ++d)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t f = FP4 ? (D / 8) * g + 2 * d + (e >> 1) : 16 * d + g + 8 * (e >> 1);
+                float* at = patch + (nt * 8 + 2 * t4 + (e & 1)) * PD + f;
+                *at = w == 3 ? o[d][nt][e] : *at + o[d][nt][e];
+              }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      const bool complete = cnt == n;
+      // the CTA's first piece starts where its run does: its slot is the even one, a later (then last) piece's the odd one
+      const uint32_t slot = 2 * blockIdx.x + (left == place[2] ? 0u : 1u);
+      const uint32_t live_rows = min(16u, p.rows - r_first);
+      for (uint32_t x = threadIdx.x; x < live_rows * (D / 4); x += 128) {
+        const uint32_t r = x / (D / 4), d4 = (x % (D / 4)) * 4;
+        float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, stat_m[w * ROWS + r]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float mw = stat_m[w * ROWS + r];
+          ll += mw == -INFINITY ? 0.0f : stat_l[w * ROWS + r] * paged_ex2(mw - mm);
+        }
+        const float4 v = *reinterpret_cast<const float4*>(patch + r * PD + d4);
+        if (complete) {
+          const float inv = ll > 0.0f ? 1.0f / ll : (ll == 0.0f ? 0.0f : ll);   // NaN stays NaN
+          const uint32_t rr = r_first + r, qi = rr / p.group, hg = rr - qi * p.group;
+          uint2* dst = reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.nq + qi) * p.heads + kvh * p.group + hg) * D + d4);
+          *dst = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+        } else {
+          float* dst = p.part + (size_t(slot) * 16 + r) * (D + 4);
+          *reinterpret_cast<float4*>(dst + d4) = v;
+          if (d4 == 0) { dst[D] = mm; dst[D + 1] = ll; }
+        }
+      }
+      // the CTA that holds an item's first tile tells the join where its pieces are
+      if (i0 == 0 && threadIdx.x == 0) {
+        const uint32_t rest = n - cnt;
+        p.meta[size_t(b) * items + item] = make_uint4(slot, 1u + (rest + per - 1) / per, blockIdx.x, 0u);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");       // patch and statistics are free for the next piece
+    }
+    if (!ok) break;
+    left -= cnt;
+    skip += cnt;
+  }
+}
+
+// out = sum over pieces, in tile order. One block per query row: groups of D / 4 threads (four values each) walk the pieces.
+template <int D>
+__global__ void __launch_bounds__(128)
+paged_join_kernel(const __grid_constant__ DecodeParams p) {
+  constexpr int LANES = D / 4, GROUPS = 128 / LANES;      // float4 lanes of a row, pieces in flight
+  __shared__ float acc_s[GROUPS][D];
+  __shared__ float l_s[GROUPS];
+  mb_grid_dependency_sync();
+  const uint32_t h = blockIdx.x % p.heads, qi = (blockIdx.x / p.heads) % p.nq, b = blockIdx.x / (p.heads * p.nq);
+  const uint32_t kvh = h / p.group, r = qi * p.group + (h - kvh * p.group), items = p.c.kv_heads * p.row_tiles;
+  int len;
+  const PagedSpan span = decode_span(p.c, b, p.nq, len);
+  __nv_bfloat16* dst = p.out + size_t(blockIdx.x) * D;
+  if (threadIdx.x == 0 && paged_len_bad(p.c, b)) paged_raise(p.c, b);
+  if (span.count() == 0 || len - int(p.nq) + int(qi) < 0) {
+    for (uint32_t d = threadIdx.x; d < D; d += 128) dst[d] = __float2bfloat16_rn(0.0f);
+    return;
+  }
+  const uint4 meta = p.meta[size_t(b) * items + kvh * p.row_tiles + r / 16];
+  const uint32_t pieces = meta.y;
+  if (pieces == 1) return;
+  const float* row = p.part + size_t(r % 16) * (D + 4);
+  auto slot_of = [&](uint32_t i) { return size_t(i == 0 ? meta.x : 2 * (meta.z + i)) * 16 * (D + 4); };
+  float mm = -INFINITY;
+  for (uint32_t i = threadIdx.x & 31; i < pieces; i += 32) mm = fmaxf(mm, row[slot_of(i) + D]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
+  const uint32_t lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float ll = 0.0f;
+#pragma unroll 4
+  for (uint32_t i = grp; i < pieces; i += GROUPS) {
+    const float* src = row + slot_of(i);
+    const float mw = src[D], f = mw == -INFINITY ? 0.0f : exp2f(mw - mm);
+    const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
+    acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+    ll = fmaf(src[D + 1], f, ll);
+  }
+  *reinterpret_cast<float4*>(&acc_s[grp][lane * 4]) = acc;
+  if (lane == 0) l_s[grp] = ll;
+  __syncthreads();
+  for (uint32_t d = threadIdx.x; d < D; d += 128) {
+    float v = 0.0f, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < GROUPS; ++i) { v += acc_s[i][d]; sum += l_s[i]; }
+    dst[d] = __float2bfloat16_rn(sum == 0.0f ? 0.0f : v / sum);
+  }
+}
+
+template <int D, bool FP4, int NT>
+int launch_decode(mb_ctx* ctx, cudaStream_t stream, const DecodeParams& p, uint32_t grid, uint32_t once_bit) {
+  using Shape = DecodeShape<D, FP4, NT>;
+  if (!(ctx->paged_once.load(std::memory_order_acquire) & once_bit)) {
+    MB_CUDA_OK(ctx, cudaFuncSetAttribute(paged_decode_kernel<D, FP4, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+    ctx->paged_once.fetch_or(once_bit, std::memory_order_release);
+  }
+  MB_CUDA_OK(ctx, mb_launch_pdl(paged_decode_kernel<D, FP4, NT>, dim3(grid), dim3(Shape::THREADS), Shape::SMEM, stream, p));
+  MB_CUDA_OK(ctx, mb_launch_pdl(paged_join_kernel<D>, dim3(p.c.batch * p.nq * p.heads), dim3(128), 0, stream, p));
+  return MB_OK;
+}
+
+uint32_t decode_grid(const mb_ctx* ctx, bool fp4, bool wide) {
+  const int sms = ctx->sm_limit > 0 ? ctx->sm_limit : ctx->sm_count;
+  return uint32_t(sms) * uint32_t(fp4 ? (wide ? 3 : 4) : 2);
+}
+size_t decode_meta_bytes(const mb_paged_kv* kv, size_t rows) {
+  return (kv->batch * kv->kv_heads * ((rows + 15) / 16) * sizeof(uint4) + 255) / 256 * 256;
+}
+
+}  // namespace
+
+MB_API size_t mb_paged_decode_workspace(mb_ctx* ctx, const mb_paged_kv* kv, size_t nq, size_t heads) {
+  if (!ctx || !kv || kv->kv_heads == 0 || heads % kv->kv_heads != 0) return 0;
+  const size_t rows = nq * (heads / kv->kv_heads);
+  // the most CTAs any variant launches, whatever the SM limit is at the call
+  return decode_meta_bytes(kv, rows) + size_t(ctx->sm_count) * 4 * 2 * 16 * (kv->d + 4) * sizeof(float);
+}
+
+MB_API int mb_paged_decode(mb_ctx* ctx, mb_stream stream_, const void* q, size_t nq, size_t heads, const mb_paged_kv* kv,
+                           const mb_score_terms* terms, void* out, void* workspace, size_t workspace_bytes) {
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  DecodeParams p;
+  MB_REQUIRE(ctx, ctx && terms, "paged_decode: null argument");
+  int rc = paged_view(ctx, "paged_decode", kv, terms, heads, &p.c);
+  if (rc) return rc;
+  MB_REQUIRE(ctx, q && out && mb_aligned(q, 16) && mb_aligned(out, 16), "paged_decode: q and out need 16-byte alignment");
+  MB_REQUIRE(ctx, nq > 0 && nq <= 1024 && kv->batch * nq * heads < (1ull << 31),
+             "paged_decode: 1 to 1024 tokens per sequence, got %zu (longer blocks: mb_paged_prompt)", nq);
+  const size_t line = (kv->table_width * kv->page_size / BC + 2) * kv->kv_heads * ((nq * (heads / kv->kv_heads) + 15) / 16);
+  MB_REQUIRE(ctx, line < (1ull << 31), "paged_decode: %zu tiles in one sequence", line);
+  const size_t need = mb_paged_decode_workspace(ctx, kv, nq, heads);
+  MB_REQUIRE(ctx, workspace && workspace_bytes >= need && mb_aligned(workspace, 256),
+             "paged_decode: needs %zu workspace bytes, 256-byte aligned", need);
+  const bool fp4 = kv->elem == MB_KV_NVFP4;
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.k = static_cast<const uint8_t*>(kv->k); p.v = static_cast<const uint8_t*>(kv->v);
+  p.ks = static_cast<const uint8_t*>(kv->k_scales); p.vs = static_cast<const uint8_t*>(kv->v_scales);
+  p.slopes = terms->slopes;
+  p.nq = uint32_t(nq); p.heads = uint32_t(heads); p.group = uint32_t(heads / kv->kv_heads);
+  p.rows = p.nq * p.group;
+  p.row_tiles = (p.rows + 15) / 16;
+  p.meta = static_cast<uint4*>(workspace);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + decode_meta_bytes(kv, p.rows));
+  p.scale = terms->scale;
+  p.scale_log2 = terms->scale * 1.4426950408889634f;
+  p.cap_log2 = terms->softcap * 1.4426950408889634f;
+  p.inv_cap = terms->softcap > 0.0f ? terms->scale / terms->softcap : 0.0f;
+  p.flags = ctx->flags_dev;
+  p.box_rows = paged_box_rows(kv->page_size, BC);
+  if (!fp4) {
+    rc = paged_pool_map(ctx, &p.tmap_k, kv->k, kv, p.box_rows);
+    if (rc) return rc;
+    rc = paged_pool_map(ctx, &p.tmap_v, kv->v, kv, p.box_rows);
+    if (rc) return rc;
+  } else {
+    memset(&p.tmap_k, 0, sizeof p.tmap_k);
+    memset(&p.tmap_v, 0, sizeof p.tmap_v);
+  }
+  const bool wide = p.rows > 8;
+  const uint32_t grid = decode_grid(ctx, fp4, wide);
+#define MB_DECODE(DD, F, N, BIT) rc = launch_decode<DD, F, N>(ctx, stream, p, grid, 1u << (BIT))
+  if (kv->d == 128) {
+    if (fp4) { if (wide) MB_DECODE(128, true, 2, 0); else MB_DECODE(128, true, 1, 1); }
+    else { if (wide) MB_DECODE(128, false, 2, 2); else MB_DECODE(128, false, 1, 3); }
+  } else {
+    if (fp4) { if (wide) MB_DECODE(64, true, 2, 4); else MB_DECODE(64, true, 1, 5); }
+    else { if (wide) MB_DECODE(64, false, 2, 6); else MB_DECODE(64, false, 1, 7); }
+  }
+#undef MB_DECODE
+  if (rc) return rc;
+  MB_LAUNCH_OK(ctx);
+  return MB_OK;
+}

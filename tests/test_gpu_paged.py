@@ -1,0 +1,440 @@
+"""GPU tests of the paged cache: append with rotation, decode and prompt attention, against plain implementations in
+64 bits on the values the device holds.
+
+Tolerances. Rounding to bf16 is off by at most 2^-8 of the value (finfo(bf16).eps / 2).
+* rotation: the 32-bit result differs from the exact one by a few 2^-24 of |x| + |y| and is rounded once, so an element is
+  off by at most 2^-8 of itself plus 4 * 2^-24 * (|x| + |y|).
+* attention: probabilities are rounded to 16 bits (2^-8 of each in bf16) before the product with V, whose sums and
+  denominators are f32, and the result once more. With p_j the exact probabilities that is at most
+  2^-8 * A + 2^-8 |o| per element, A = sum_j p_j |v_j|; the f32 terms (2^-22 relative in the exponentials, scores of up
+  to 128 products with unit roundoff 2^-24 of sum |q||k|, tanh to 2^-22 of the cap) stay below a tenth of that for the
+  scores of these tests (up to about 60), so 1.1 * (2^-8 * A + 2^-8 |o|) bounds every element.
+"""
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def pg():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    torch.cuda.set_device(0)
+    from maryml_b200 import paged
+    return paged
+
+
+# ---- plain forms ---------------------------------------------------------------------------
+_E2M1 = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+def fp4_values(codes, scales):
+    table = torch.tensor(_E2M1 + [-x for x in _E2M1], dtype=torch.float64, device=codes.device)
+    pair = torch.stack((codes & 15, codes >> 4), dim=-1).int()
+    v = table[pair].reshape(*codes.shape[:-1], codes.shape[-1] // 8, 16)
+    return (v * scales.view(torch.float8_e4m3fn).double().unsqueeze(-1)).flatten(-2)
+
+
+class Setup:
+    """A pool with every sequence's rows scattered over it; whatever no sequence owns is poison."""
+
+    def __init__(self, pg, lens, page, kv_heads, d, nvfp4=False, seed=0, spare=3, poison=True, width=None):
+        g = torch.Generator(device="cuda").manual_seed(1000 + seed)
+        self.lens_host = list(lens)
+        self.page, self.kvh, self.d, self.nvfp4 = page, kv_heads, d, nvfp4
+        need = [-(-n // page) for n in lens]
+        pages = sum(need) + spare
+        perm = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+        width = width or max(max(need), 1) + 2
+        table = np.full((len(lens), width), -7, dtype=np.int32)
+        at = 0
+        for b, n in enumerate(need):
+            table[b, :n] = perm[at:at + n]
+            at += n
+        self.table = torch.from_numpy(table).cuda()
+        self.lens = torch.tensor(self.lens_host, dtype=torch.int32, device="cuda")
+        if nvfp4:
+            mk = lambda: torch.randint(0, 256, (pages, page, kv_heads * d // 2), dtype=torch.uint8, device="cuda", generator=g)
+            ms = lambda: torch.randint(0x28, 0x34, (pages, page, kv_heads * d // 16), dtype=torch.uint8, device="cuda", generator=g)
+            planes = [mk(), mk(), ms(), ms()]
+        else:
+            mk = lambda: torch.randn((pages, page, kv_heads, d), device="cuda", generator=g).to(torch.bfloat16)
+            planes = [mk(), mk()]
+        if poison:
+            keep = torch.zeros(pages * page, dtype=torch.bool)
+            for b, n in enumerate(self.lens_host):
+                r = torch.arange(n)
+                keep[torch.from_numpy(table[b].astype(np.int64))[r // page] * page + r % page] = True
+            gone = (~keep).cuda().view(pages, page)
+            for t in planes[:2] if not nvfp4 else planes[2:]:
+                t[gone] = float("nan") if not nvfp4 else 0x7F          # NaN rows; NaN scales
+        self.cache = pg.PagedCache(planes[0], planes[1], *(planes[2:] or (None, None)), head_dim=d)
+        self.gen = g
+
+    def rows(self, b, name):
+        """[len, kv_heads, d] in 64 bits."""
+        n = self.lens_host[b]
+        r = torch.arange(n, device="cuda")
+        at = self.table[b].long()[r // self.page] * self.page + r % self.page
+        if not self.nvfp4:
+            return getattr(self.cache, name).reshape(-1, self.kvh, self.d)[at].double()
+        codes = getattr(self.cache, name).reshape(-1, self.kvh * self.d // 2)[at]
+        scales = getattr(self.cache, name + "_scales").reshape(-1, self.kvh * self.d // 16)[at]
+        return fp4_values(codes, scales).view(n, self.kvh, self.d)
+
+
+def plain_attention(q, k, v, pos, scale, softcap=0.0, window=0, slopes=None, prefix=0):
+    """q [n, heads, d] at positions pos [n]; k, v [len, kv_heads, d], all 64 bits -> (o, A) with A = sum p |v|."""
+    n, heads, d = q.shape
+    length, kvh, _ = k.shape
+    group = heads // kvh
+    o, a = torch.zeros_like(q), torch.zeros_like(q)
+    if length == 0:
+        return o, a
+    kpos = torch.arange(length, device=q.device)
+    away = pos[:, None] - kpos[None]
+    seen = away >= 0
+    if window:
+        seen &= away < window
+    seen |= (kpos < prefix)[None]
+    seen &= (pos >= 0)[:, None]
+    for h in range(heads):
+        x = q[:, h] @ k[:, h // group].t() * scale
+        if softcap:
+            x = softcap * torch.tanh(x / softcap)
+        if slopes is not None:
+            x = x - slopes[h].double() * away.abs()
+        x = torch.where(seen, x, torch.full_like(x, -math.inf))
+        p = torch.nan_to_num(torch.softmax(x, -1), nan=0.0)
+        o[:, h], a[:, h] = p @ v[:, h // group], p @ v[:, h // group].abs()
+    return o, a
+
+
+def check_attention(got, want, a):
+    assert torch.isfinite(got.float()).all()
+    err, room = (got.double() - want).abs(), 1.1 * 2.0 ** -8 * (a + want.abs()) + 1e-30
+    worst = (err / room).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, worst
+    return worst
+
+
+def terms_of(s, heads, batch, softcap=0.0, window=0, slopes=False, prefix=None):
+    kw = {"softcap": softcap, "window": window}
+    if slopes:
+        kw["slopes"] = torch.exp2(-8.0 * torch.arange(1, heads + 1, device="cuda", dtype=torch.float32) / heads)
+    if prefix is not None:
+        kw["prefix"] = torch.tensor([prefix + 3 * b for b in range(batch)], dtype=torch.int32, device="cuda")
+    return kw
+
+
+def plain_terms(kw, b):
+    return {"softcap": kw["softcap"], "window": kw["window"], "slopes": kw.get("slopes"),
+            "prefix": int(kw["prefix"][b]) if "prefix" in kw else 0}
+
+
+def run_decode(pg, s, heads, nq, gain=1.0, **t):
+    batch = len(s.lens_host)
+    q = (torch.randn((batch, nq, heads, s.d), device="cuda", generator=s.gen) * gain).to(torch.bfloat16)
+    kw = terms_of(s, heads, batch, **t)
+    got = pg.paged_attention_decode(q, s.cache, s.table, s.lens, **kw)
+    torch.cuda.synchronize()
+    worst = 0.0
+    for b, n in enumerate(s.lens_host):
+        pos = torch.arange(n - nq, n, device="cuda")
+        o, a = plain_attention(q[b].double(), s.rows(b, "k"), s.rows(b, "v"), pos, 1.0 / math.sqrt(s.d), **plain_terms(kw, b))
+        worst = max(worst, check_attention(got[b], o, a))
+    return got, worst
+
+
+def no_flags(pg):
+    rc, flags = pg.context(0).check_flags()
+    assert rc == 0, flags
+
+
+# ---- decode ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("nvfp4", [False, True])
+@pytest.mark.parametrize("lens,page,heads,kvh,d,nq", [
+    ([1], 16, 8, 8, 128, 1),                            # one row, one query head per KV head
+    ([64, 0, 1, 63, 65], 16, 8, 2, 128, 1),             # around a tile, and an empty sequence
+    ([200, 777, 4, 1025], 48, 32, 8, 128, 1),           # pages that end inside tiles, several pieces
+    ([5000], 64, 4, 1, 128, 1),                         # one KV head: the row is cut over many CTAs
+    ([130, 2047, 300], 256, 16, 2, 64, 1),              # head_dim 64, all eight columns live
+    ([33, 500], 80, 10, 1, 64, 1),                      # ten query heads over one KV head: two N tiles
+    ([40, 900], 32, 48, 2, 128, 1),                     # twenty-four: two row tiles
+    ([7, 128, 2, 600], 128, 8, 2, 128, 3),              # three tokens; a sequence shorter than that
+    ([300, 9], 16, 5, 5, 64, 5),
+])
+def test_decode(pg, lens, page, heads, kvh, d, nq, nvfp4):
+    run_decode(pg, Setup(pg, lens, page, kvh, d, nvfp4, seed=len(lens) + page), heads, nq)
+    no_flags(pg)
+
+
+@pytest.mark.parametrize("nvfp4", [False, True])
+@pytest.mark.parametrize("terms", [
+    {"softcap": 20.0}, {"window": 1}, {"window": 100}, {"window": 64, "prefix": 5}, {"slopes": True},
+    {"softcap": 30.0, "window": 333, "prefix": 130, "slopes": True}, {"prefix": 10000}, {"window": 1 << 40},
+])
+def test_decode_terms(pg, terms, nvfp4):
+    for d, heads, kvh, nq in ((128, 8, 2, 1), (64, 6, 1, 2), (128, 32, 2, 1)):
+        run_decode(pg, Setup(pg, [700, 64, 129, 1, 0], 32, kvh, d, nvfp4, seed=nq), heads, nq, gain=4.0, **terms)
+    no_flags(pg)
+
+
+def test_decode_of_many_sequences_and_one_long_one(pg):
+    """Lengths that differ by four orders of magnitude share the line of tiles; more than 32 sequences need the second
+    round of the search for a CTA's first tile."""
+    lens = [(37 * i) % 150 for i in range(100)] + [20000] + [1] * 30
+    run_decode(pg, Setup(pg, lens, 64, 2, 128, seed=5), 8, 1)
+    no_flags(pg)
+
+
+def test_decode_evicted_pages_below_the_window_are_not_touched(pg):
+    for nvfp4 in (False, True):
+        s = Setup(pg, [1000, 555], 16, 2, 128, nvfp4, seed=3)
+        q = torch.randn((2, 1, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16)
+        want = pg.paged_attention_decode(q, s.cache, s.table, s.lens, window=100)
+        cut = s.table.clone()
+        cut[0, :(1000 - 100) // 16] = -1
+        cut[1, :(555 - 100) // 16] = 1 << 30
+        got = pg.paged_attention_decode(q, s.cache, cut, s.lens, window=100)
+        assert torch.equal(got, want)
+    no_flags(pg)
+
+
+def test_decode_repeats_its_bits(pg):
+    s = Setup(pg, [4097, 60, 1900, 4097], 16, 2, 128, seed=11)
+    q = torch.randn((4, 1, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16)
+    ref = pg.paged_attention_decode(q, s.cache, s.table, s.lens).clone()
+    for _ in range(200):
+        assert torch.equal(pg.paged_attention_decode(q, s.cache, s.table, s.lens), ref)
+
+
+# ---- prompt ------------------------------------------------------------------------------------
+def run_prompt(pg, s, heads, q_len, gain=1.0, pad=0, **t):
+    batch, total = len(q_len), sum(q_len) + pad
+    q = (torch.randn((total, heads, s.d), device="cuda", generator=s.gen) * gain).to(torch.bfloat16)
+    cu = torch.tensor([0] + list(np.cumsum(q_len)), dtype=torch.int32, device="cuda")
+    kw = terms_of(s, heads, batch, **t)
+    out = torch.full_like(q, 7.0)
+    got = pg.paged_attention_prompt(q, cu, s.cache, s.table, s.lens, out=out, **kw)
+    torch.cuda.synchronize()
+    assert got is out and (got[sum(q_len):] == 7.0).all()
+    worst, t0 = 0.0, 0
+    for b, n in enumerate(q_len):
+        pos = torch.arange(s.lens_host[b] - n, s.lens_host[b], device="cuda")
+        o, a = plain_attention(q[t0:t0 + n].double(), s.rows(b, "k"), s.rows(b, "v"), pos, 1.0 / math.sqrt(s.d), **plain_terms(kw, b))
+        worst = max(worst, check_attention(got[t0:t0 + n], o, a))
+        t0 += n
+    return got, worst
+
+
+PROMPTS = [
+    # lens, q_len, page, heads, kvh, d
+    ([1], [1], 16, 4, 1, 128),
+    ([128], [128], 128, 1, 1, 128),                               # one tile, one head
+    ([300, 5, 64], [300, 5, 64], 16, 8, 2, 128),                  # fresh ragged prompts, pages of 16
+    ([1000, 0, 777, 130], [200, 0, 1, 130], 48, 32, 8, 128),      # chunks over a past, an empty one
+    ([260, 700], [260, 99], 256, 10, 2, 128),                     # five heads per KV head: 125 of 128 rows in use
+    ([513, 64], [513, 10], 32, 16, 4, 64),
+    ([2000], [7], 64, 4, 4, 64),                                  # few blocks over many rows: the keys are cut
+    ([3000, 40], [33, 20], 80, 4, 1, 128),
+    ([90], [90], 16, 128, 1, 64),                                 # one token per tile
+]
+
+
+@pytest.mark.parametrize("nvfp4", [False, True])
+@pytest.mark.parametrize("lens,q_len,page,heads,kvh,d", PROMPTS)
+def test_prompt(pg, lens, q_len, page, heads, kvh, d, nvfp4):
+    run_prompt(pg, Setup(pg, lens, page, kvh, d, nvfp4, seed=page + d), heads, q_len, pad=2)
+    no_flags(pg)
+
+
+@pytest.mark.parametrize("nvfp4", [False, True])
+@pytest.mark.parametrize("terms", [
+    {"softcap": 20.0}, {"window": 1}, {"window": 100}, {"window": 200, "prefix": 5}, {"slopes": True},
+    {"softcap": 30.0, "window": 333, "prefix": 130, "slopes": True}, {"prefix": 10000}, {"prefix": 300, "slopes": True},
+    {"window": 1 << 40},
+])
+def test_prompt_terms(pg, terms, nvfp4):
+    for d, heads, kvh in ((128, 8, 2), (64, 6, 1)):
+        run_prompt(pg, Setup(pg, [900, 64, 400, 1, 0], 32, kvh, d, nvfp4, seed=d), heads, [300, 64, 129, 1, 0], gain=4.0, **terms)
+    run_prompt(pg, Setup(pg, [2500], 16, 1, 128, nvfp4, seed=8), 4, [40], gain=4.0, **terms)       # keys cut over CTAs
+    no_flags(pg)
+
+
+def test_prompt_scores_that_outgrow_their_reference(pg):
+    """Keys whose scores rise by more than 2^40 towards the sequence's start, the last tiles to be read: every tile moves
+    the running reference and rescales the output. The queries and keys are such that scores are exact."""
+    for d in (64, 128):
+        s = Setup(pg, [1500], 64, 1, d, seed=1, poison=False)
+        k = s.cache.k.view(-1, d)
+        rows = torch.arange(1500, device="cuda")
+        at = s.table[0].long()[rows // 64] * 64 + rows % 64
+        k[at] = 0
+        step = (1500 - rows).float() // 32
+        k[at, 0] = step.to(torch.bfloat16)                        # at most 46: exact
+        q = torch.zeros((700, 2, d), device="cuda", dtype=torch.bfloat16)
+        q[:, 0, 0], q[:, 1, 0] = 16.0, -16.0
+        cu = torch.tensor([0, 700], dtype=torch.int32, device="cuda")
+        got = pg.paged_attention_prompt(q, cu, s.cache, s.table, s.lens, scale=1.0)
+        o, a = plain_attention(q.double(), s.rows(0, "k"), s.rows(0, "v"), torch.arange(800, 1500, device="cuda"), 1.0)
+        check_attention(got, o, a)
+    no_flags(pg)
+
+
+def test_prompt_matches_decode_token_by_token(pg):
+    s = Setup(pg, [300, 45], 16, 2, 128, seed=6)
+    q = torch.randn((2, 1, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16)
+    a = pg.paged_attention_decode(q, s.cache, s.table, s.lens)
+    b = pg.paged_attention_prompt(q.view(2, 8, 128), torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"), s.cache, s.table, s.lens)
+    assert (a.view(2, 8, 128).float() - b.float()).abs().max() <= 2.0 ** -6 * a.float().abs().max()
+
+
+# ---- append ----------------------------------------------------------------------------------
+def plain_rotate(x, pos, inv_freq, sections=None):
+    """x [n, heads, d] 64 bits; pos [axes, n] -> (rotated, |x| + |y| per element)."""
+    d = x.shape[-1]
+    f = inv_freq.double()
+    if sections is None:
+        angle = pos[0].double()[:, None] * f
+    else:
+        axis = np.repeat(np.arange(len(sections)), sections)
+        angle = torch.stack([pos[int(a)].double() * f[i] for i, a in enumerate(axis)], dim=1)
+    c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+    lo, hi = x[..., :d // 2], x[..., d // 2:]
+    size = (lo.abs() + hi.abs()).repeat(1, 1, 2)
+    return torch.cat((lo * c - hi * s, hi * c + lo * s), -1), size
+
+
+def inv_freq_of(d, theta=1e6):
+    f = np.arange(d // 2, dtype=np.float64)
+    return torch.from_numpy((1.0 / theta ** (2.0 * f / d)).astype(np.float32)).cuda()
+
+
+def run_append(pg, s, hq, q_len, axes=0, ragged=True, far=0, pad=0, stride=0):
+    """Appends q_len[b] tokens as the last rows of each sequence and checks queries, rows and untouched bytes."""
+    d, kvh = s.d, s.kvh
+    total = sum(q_len) + pad
+    heads = hq + 2 * kvh
+    wide = torch.randn((total, heads * d + stride), device="cuda", generator=s.gen).to(torch.bfloat16)
+    qkv = wide[:, :heads * d]
+    f = inv_freq_of(d)
+    cu = torch.tensor([0] + list(np.cumsum(q_len)), dtype=torch.int32, device="cuda") if ragged else None
+    kw = {}
+    sections = None
+    if axes:
+        kw["positions"] = torch.randint(-50, 100000 + far, (axes, total), dtype=torch.int32, device="cuda", generator=s.gen)
+        if axes > 1:
+            left = d // 2
+            sections = [left // axes + (1 if a < left % axes else 0) for a in range(axes)]
+            kw["sections"] = tuple(sections)
+    planes = {n: getattr(s.cache, n) for n in ("k", "v", "k_scales", "v_scales") if getattr(s.cache, n) is not None}
+    before = {n: t.clone() for n, t in planes.items()}
+    out = torch.full((total, hq, d), 7.0, dtype=torch.bfloat16, device="cuda")
+    got = pg.paged_append(qkv, s.cache, s.table, s.lens, f, cu_q=cu, out=out, **kw)
+    torch.cuda.synchronize()
+    assert got.data_ptr() == out.data_ptr()
+    x = qkv.double().reshape(total, heads, d)
+    t0 = 0
+    touched = torch.zeros(s.cache.pages * s.page, dtype=torch.bool, device="cuda")
+    for b, n in enumerate(q_len):
+        row = torch.arange(s.lens_host[b] - n, s.lens_host[b], device="cuda")
+        pos = kw["positions"][:, t0:t0 + n] if axes else row[None]
+        rot, size = plain_rotate(x[t0:t0 + n, :hq + kvh], pos, f, sections)
+        room = 2.0 ** -8 * rot.abs() + 4 * 2.0 ** -24 * size + 1e-30
+        assert ((got[t0:t0 + n].double() - rot[:, :hq]).abs() <= room[:, :hq]).all()
+        at = s.table[b].long()[row // s.page] * s.page + row % s.page
+        touched[at] = True
+        if not s.nvfp4:
+            k = s.cache.k.reshape(-1, kvh, d)[at].double()
+            assert ((k - rot[:, hq:]).abs() <= room[:, hq:]).all()
+            assert torch.equal(s.cache.v.reshape(-1, kvh, d)[at], qkv.reshape(total, heads, d)[t0:t0 + n, hq + kvh:])
+        t0 += n
+    assert (got[t0:] == 7.0).all()
+    for n, t in planes.items():
+        same = (t.reshape(len(touched), -1).view(torch.uint8) == before[n].reshape(len(touched), -1).view(torch.uint8)).all(1)
+        assert same[~touched].all(), n
+    return qkv, got, touched, kw, cu
+
+
+@pytest.mark.parametrize("lens,q_len,page,hq,kvh,d", [
+    ([1], [1], 16, 4, 1, 128),
+    ([300, 17, 5], [1, 1, 1], 16, 8, 2, 128),
+    ([300, 17, 5, 64], [40, 0, 5, 64], 48, 5, 5, 64),
+    ([2000, 900], [1500, 333], 128, 32, 8, 128),
+    ([700, 0, 650], [700, 0, 650], 80, 7, 1, 64),
+])
+@pytest.mark.parametrize("axes", [0, 1, 3, 4])
+def test_append(pg, lens, q_len, page, hq, kvh, d, axes):
+    run_append(pg, Setup(pg, lens, page, kvh, d, seed=page), hq, q_len, axes, pad=3, stride=8 * axes)
+    no_flags(pg)
+
+
+def test_append_uniform_without_cu_q(pg):
+    run_append(pg, Setup(pg, [5, 77, 130], 16, 2, 128, seed=2), 8, [4, 4, 4], ragged=False)
+    no_flags(pg)
+
+
+def test_append_far_positions(pg):
+    """At a million rows the angle of the first frequency has lost six bits in f32; the kernel's has not."""
+    run_append(pg, Setup(pg, [50], 16, 2, 128, seed=2), 4, [50], axes=1, far=2 ** 31 - 200000)
+
+
+@pytest.mark.parametrize("d,kvh,page,q_len", [(128, 2, 32, [70, 1, 300]), (64, 3, 16, [1, 1, 1]), (128, 8, 64, [900, 300, 17])])
+def test_append_nvfp4_rows_are_the_quantized_bf16_rows(pg, d, kvh, page, q_len):
+    """Bit for bit: the bytes quantize_kv_rows gives for the rows a bf16 cache receives."""
+    from maryml_b200.attention import quantize_kv_rows
+    lens = [n + 11 * i for i, n in enumerate(q_len)]
+    s4 = Setup(pg, lens, page, kvh, d, nvfp4=True, seed=4)
+    qkv, got, touched, kw, cu = run_append(pg, s4, 4, q_len, axes=3)
+    s16 = Setup(pg, lens, page, kvh, d, seed=4)
+    assert torch.equal(s16.table, s4.table)
+    q16 = pg.paged_append(qkv, s16.cache, s16.table, s16.lens, inv_freq_of(d), cu_q=cu, **kw)
+    assert torch.equal(q16, got[:q16.shape[0]])
+    for name in ("k", "v"):
+        rows = getattr(s16.cache, name).reshape(-1, kvh, d)[touched].unsqueeze(0).contiguous()
+        codes, scales = quantize_kv_rows(rows)
+        assert torch.equal(getattr(s4.cache, name).reshape(-1, kvh * d // 2)[touched], codes[0])
+        assert torch.equal(getattr(s4.cache, name + "_scales").reshape(-1, kvh * d // 16)[touched], scales[0])
+
+
+# ---- bad tables and lengths -----------------------------------------------------------------------
+@pytest.mark.parametrize("nvfp4", [False, True])
+def test_bad_entries_are_contained_and_flagged(pg, nvfp4):
+    s = Setup(pg, [100, 90, 80], 16, 2, 128, nvfp4, seed=9, poison=False)
+    q = torch.randn((3, 1, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16)
+    want = pg.paged_attention_decode(q, s.cache, s.table, s.lens).clone()
+    no_flags(pg)
+    bad = s.table.clone()
+    bad[1, 2] = -5
+    got = pg.paged_attention_decode(q, s.cache, bad, s.lens)
+    rc, flags = pg.context(0).check_flags()
+    assert rc != 0 and flags[2] == 2
+    assert torch.equal(got[0], want[0]) and torch.equal(got[2], want[2]) and torch.isfinite(got.float()).all()
+    # the page reads as zeros
+    k, v = s.rows(1, "k"), s.rows(1, "v")
+    k[32:48], v[32:48] = 0, 0
+    o, a = plain_attention(q[1].double(), k, v, torch.tensor([89], device="cuda"), 1 / math.sqrt(128))
+    check_attention(got[1], o, a)
+    # lengths beyond the table are clamped to it (the entries it has there are no pages), negative ones to zero
+    for value in (10 ** 9, -4):
+        lens = s.lens.clone()
+        lens[2] = value
+        got = pg.paged_attention_decode(q, s.cache, s.table, lens)
+        rc, flags = pg.context(0).check_flags()
+        assert rc != 0 and flags[2] == 3, flags
+        assert torch.equal(got[:2], want[:2]) and torch.isfinite(got.float()).all()
+        assert value > 0 or (got[2] == 0).all()
+    # an append has nowhere to go: nothing is written
+    planes = [t for t in (s.cache.k, s.cache.v, s.cache.k_scales, s.cache.v_scales) if t is not None]
+    before = [t.clone() for t in planes]
+    qkv = torch.randn((3, 12 * 128), device="cuda", generator=s.gen).to(torch.bfloat16)
+    bad = torch.full_like(s.table, s.cache.pages)
+    pg.paged_append(qkv, s.cache, bad, s.lens, inv_freq_of(128))
+    rc, flags = pg.context(0).check_flags()
+    assert rc != 0 and flags[2] in (1, 2, 3)
+    assert all(torch.equal(t, u) for t, u in zip(planes, before))
