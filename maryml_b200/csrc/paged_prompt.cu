@@ -86,6 +86,21 @@ __device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// tanh of two values with |x| <= 1: x + x^3 q(x^2), q of degree four, off by 3.3e-7 at most (a weighted
+// least-squares fit, reweighted towards the smallest maximum). As exact as paged_tanh in the absolute error that counts, and without its two special-function operations.
+__device__ __forceinline__ f32x2 tanh_pair(f32x2 x) {
+  const f32x2 y = f2_mul(x, x);
+  f32x2 q = f2_fma(f2_pack(-2.983081579e-03f, -2.983081579e-03f), y, f2_pack(1.653281572e-02f, 1.653281572e-02f));
+  q = f2_fma(q, y, f2_pack(-5.142535359e-02f, -5.142535359e-02f));
+  q = f2_fma(q, y, f2_pack(1.327561524e-01f, 1.327561524e-01f));
+  q = f2_fma(q, y, f2_pack(-3.332866991e-01f, -3.332866991e-01f));
+  return f2_fma(f2_mul(q, y), x, x);
+}
 
 // bf16 A and B, f32 accumulate, M = 128, N = n; B either K-major (0) or MN-major (1).
 __host__ __device__ constexpr uint32_t idesc(uint32_t n, uint32_t b_mn_major) {
@@ -106,7 +121,7 @@ struct PromptShape {
   static constexpr int TILE = HALVES * HALF;                     // a K or V tile
   static constexpr int Q_BYTES = 2 * HALVES * QT * 128;
   static constexpr int SMEM = (KSTAGES + VSTAGES) * TILE + Q_BYTES + 1024 + 512;
-  static constexpr int THREADS = FP4 ? 416 : 384;
+  static constexpr int THREADS = FP4 ? 512 : 384;
   static constexpr int LOADERS = FP4 ? 4 : 1;                    // arrivals on a full barrier
 };
 
@@ -149,7 +164,7 @@ __device__ __forceinline__ BlockPlace find_block(const PromptParams& p, uint32_t
   return at;
 }
 
-template <int D, bool FP4>
+template <int D, bool FP4, bool CAPPED, bool BIASED>
 __global__ void __launch_bounds__(PromptShape<D, FP4>::THREADS, 1)
 paged_prompt_kernel(const __grid_constant__ PromptParams p) {
   using Shape = PromptShape<D, FP4>;
@@ -238,7 +253,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
   const uint32_t n_tiles = min(per, all_tiles - i_first);
   const int tile_tokens = int(p.tile_tokens);
 
-  const bool loader = FP4 ? (warp == 0 || warp == 2 || warp == 3 || warp == 12) : warp == 0;
+  const bool loader = warp == 0 || warp >= 12;
   if (loader && n_tiles > 0) {
     if (warp == 0) {
       if (elect_one()) {
@@ -252,7 +267,9 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
       }
       __syncwarp();
     }
-    if (!FP4) {
+    if (FP4 && warp == 0) {
+      // the queries are all it loads
+    } else if (!FP4) {
       // ------------------------------ producer: tiles by TMA ------------------------------
       const uint32_t per_tile = BC / p.box_rows;
       auto pages_of = [&](uint32_t box) -> uint32_t {
@@ -319,31 +336,39 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     } else {
       // ------------------------------ expanders: rows 32 e .. 32 e + 31 of a tile ------------------------------
       // A lane takes 16 bytes of codes (32 features, two scales) of a row: D / 32 lanes to a row.
-      const uint32_t e = warp == 0 ? 0u : warp == 12 ? 3u : uint32_t(warp) - 1u;
+      const uint32_t e = uint32_t(warp) - 12u;
       constexpr int PER = D / 32, CH = PER;                     // lanes per row; 16-byte loads per lane and tile
       const uint32_t q = lane % PER, row_in = lane / PER;       // rows row_in + i * (32 / PER)
       uint4 codes[CH], codes_next[CH];
       uint32_t sc[CH], sc_next[CH];
-      // loads of half-step h: K of tile h / 2 for even h, V for odd h
+      // pages of the warp's two 16-row groups of the next 16 tiles, a lane each, fetched a window ahead
+      auto pages_of = [&](uint32_t x) -> uint32_t {
+        const uint32_t i = x >> 1;
+        if (i >= n_tiles) return p.c.pages;
+        const uint32_t r = span.tile_down(i_first + i) * BC + e * 32u + (x & 1u) * 16u;
+        if (!span.needed(int(r), 16)) return p.c.pages;
+        return paged_page(p.c, b, mb_fastdiv_q(r, p.c.page_div));
+      };
+      uint32_t ids = pages_of(lane), ids_next = pages_of(32 + lane);
+      // loads of half-step h: K of tile h / 2 for even h, V for odd h; rows that are not there become zeros
       auto fetch = [&](uint32_t h, uint4* cd, uint32_t* s2) {
         const uint32_t i = h >> 1;
         if (i >= n_tiles) return;
+        if ((h & 31u) == 0 && h > 0) { ids = ids_next; ids_next = pages_of(h + 32 + lane); }
         const uint8_t* pc = (h & 1u) ? p.v : p.k;
         const uint8_t* ps = (h & 1u) ? p.vs : p.ks;
         const uint32_t r0 = span.tile_down(i_first + i) * BC + e * 32u;
 #pragma unroll
         for (int x = 0; x < CH; ++x) {
-          const uint32_t r = r0 + row_in + x * (32 / PER), g16 = r & ~15u;
+          const uint32_t in = row_in + x * (32 / PER), r = r0 + in, r16 = r0 + (in & 16u);
+          const uint32_t page = __shfl_sync(0xFFFFFFFFu, ids, (h & 30u) + (x * (32 / PER) >= 16 ? 1u : 0u));
           cd[x] = make_uint4(0, 0, 0, 0);
           s2[x] = 0;
-          if (int(r) < len && span.needed(int(g16), 16)) {
-            const uint32_t entry = mb_fastdiv_q(r, p.c.page_div);
-            const uint32_t page = paged_page(p.c, b, entry);
-            if (page < p.c.pages) {
-              const size_t at = (size_t(page) * p.c.page_size + (r - entry * p.c.page_size)) * p.c.kv_heads + kvh;
-              cd[x] = __ldg(reinterpret_cast<const uint4*>(pc + at * (D / 2)) + q);
-              s2[x] = __ldg(reinterpret_cast<const uint16_t*>(ps + at * (D / 16)) + q);
-            }
+          if (int(r) < len && page < p.c.pages) {
+            const uint32_t in_page = r16 - mb_fastdiv_q(r16, p.c.page_div) * p.c.page_size + (in & 15u);
+            const size_t at = (size_t(page) * p.c.page_size + in_page) * p.c.kv_heads + kvh;
+            cd[x] = __ldg(reinterpret_cast<const uint4*>(pc + at * (D / 2)) + q);
+            s2[x] = __ldg(reinterpret_cast<const uint16_t*>(ps + at * (D / 16)) + q);
           }
         }
       };
@@ -460,7 +485,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
   } else if (warp >= 4 && warp < 12) {
     // ------------------------------ softmax groups: a thread per query row ------------------------------
     const int t = (warp - 4) >> 2;
-    const uint32_t quad = uint32_t(warp) & 3u, r = quad * 32u + lane;
+    const uint32_t quad = uint32_t(warp) & 3u, r = quad * 32u + lane;       // TMEM lanes of this warp, row of the tile
     const uint32_t tok_in = mb_fastdiv_q(r, p.group_div), hg = r - tok_in * p.group;
     const int tok = t * tile_tokens + int(tok_in);                // token of the block
     const bool mine = tok_in < p.tile_tokens && tok < count;      // a row of `out`
@@ -468,9 +493,8 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     const bool live = mine && qpos >= 0;
     const uint32_t lane_addr = (quad * 32u) << 16;
     const uint32_t t_s = tmem_base + lane_addr + S_COL + 128 * t, t_o = tmem_base + lane_addr + O_COL + D * t;
-    const bool capped = p.inv_cap > 0.0f, biased = p.slopes != nullptr;
-    const float mult = capped ? p.cap_log2 : p.scale_log2;
-    const float slope = biased && mine ? __ldg(p.slopes + kvh * p.group + hg) * 1.4426950408889634f : 0.0f;
+    const float mult = CAPPED ? p.cap_log2 : p.scale_log2;
+    const float slope = BIASED && mine ? __ldg(p.slopes + kvh * p.group + hg) * 1.4426950408889634f : 0.0f;
     const int window = p.c.window ? int(p.c.window) : 0x40000000;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
@@ -485,88 +509,112 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         const int vis = live ? min(len, qpos + 1) - kabs : 0;
         const int first = qpos + 1 - window - kabs;
         const int pre = live ? span.prefix - kabs : 0;
-        // nothing to mask for any row of the warp (what rows without a query hold does not matter)
-        const bool open = __all_sync(0xFFFFFFFFu, !live || (vis >= 64 && first <= 0) || (pre >= 64 && (!biased || qpos >= kabs + 63)));
-        const bool any = (min(vis, 64) > max(first, 0)) || pre > 0;
-        uint32_t sr[64];
-        tmem_ld_x32(t_s + 64 * u, sr);
-        tmem_ld_x32(t_s + 64 * u + 32, sr + 32);
-        tmem_ld_wait();
-        if (capped) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) sr[i] = __float_as_uint(paged_tanh(__uint_as_float(sr[i]) * p.inv_cap));
-        }
-        // the score of key i in units of log2, less `ref`
-        auto score = [&](int i, float ref) -> float {
-          float x = fmaf(__uint_as_float(sr[i]), mult, -ref);
-          if (biased) x = fmaf(-slope, fabsf(float(qpos - kabs - i)), x);
-          return x;
-        };
-        auto seen = [&](int i) { return (i < vis && i >= first) || i < pre; };
-        auto maximum = [&]() -> float {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < 64; ++i) mx = fmaxf(mx, seen(i) ? score(i, 0.0f) : -INFINITY);
-          return mx;
-        };
+        const bool begin = j == 0 && u == 0;
         uint32_t w[32];
         float sum = 0.0f;
-        auto probabilities = [&]() {
+        // The ordinary unit: every key seen by every row of the warp (what rows without a query hold does not matter),
+        // references at hand.
+        bool done = !begin && __all_sync(0xFFFFFFFFu, !live || (m > -INFINITY && ((vis >= 64 && first <= 0) || (pre >= 64 && (!BIASED || qpos >= kabs + 63)))));
+        if (done) {
+          uint32_t sr[64];
+          tmem_ld_x32(t_s + 64 * u, sr);
+          tmem_ld_x32(t_s + 64 * u + 32, sr + 32);
+          tmem_ld_wait();
+          const f32x2 mult2 = f2_pack(mult, mult);
+          if (CAPPED) {
+            float big = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) big = fmaxf(big, fabsf(__uint_as_float(sr[i])));
+            // scores beyond the cap are left to the general form (NaN passes here)
+            done = __all_sync(0xFFFFFFFFu, big * p.inv_cap <= 1.0f || !live);
+            const f32x2 c2 = f2_pack(p.inv_cap, p.inv_cap);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              float a0, a1;
+              f2_unpack(tanh_pair(f2_mul(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), c2)), a0, a1);
+              sr[2 * i] = __float_as_uint(a0);
+              sr[2 * i + 1] = __float_as_uint(a1);
+            }
+          }
+          // the keys are at or before the query, so the bias is linear in the key
+          const float off = BIASED ? fmaf(-slope, float(qpos - kabs), -m) : -m;
+          f32x2 off2 = f2_pack(off, off + slope);
+          const f32x2 step2 = f2_pack(2.0f * slope, 2.0f * slope);
           f32x2 acc0 = f2_pack(0.0f, 0.0f), acc1 = acc0;
-          if (open) {
-            // every key is seen and at or before the query: the bias is linear in the key, one more packed add
-            const f32x2 mult2 = f2_pack(mult, mult);
-            const float off = biased ? fmaf(-slope, float(qpos - kabs), -m) : -m;
-            f32x2 off2 = f2_pack(off, off + slope);
-            const f32x2 slope2 = f2_pack(2.0f * slope, 2.0f * slope);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              float x0, x1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), mult2, off2), x0, x1);
-              const float p0 = paged_ex2(x0), p1 = paged_ex2(x1);
-              if (i & 1) acc1 = f2_add(acc1, f2_pack(p0, p1)); else acc0 = f2_add(acc0, f2_pack(p0, p1));
-              w[i] = pack2(p0, p1);
-              if (biased) off2 = f2_add(off2, slope2);
-            }
-          } else {
-            const float ref = m == -INFINITY ? INFINITY : m;         // nothing seen yet: p = 0
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float p0 = seen(2 * i) ? paged_ex2(score(2 * i, ref)) : 0.0f;
-              const float p1 = seen(2 * i + 1) ? paged_ex2(score(2 * i + 1, ref)) : 0.0f;
-              acc0 = f2_add(acc0, f2_pack(p0, p1));
-              w[i] = pack2(p0, p1);
-            }
+          for (int i = 0; i < 32; ++i) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1])), mult2, off2), x0, x1);
+            x0 = paged_ex2(x0);
+            x1 = paged_ex2(x1);
+            if (i & 1) acc1 = f2_add(acc1, f2_pack(x0, x1)); else acc0 = f2_add(acc0, f2_pack(x0, x1));
+            w[i] = pack2(x0, x1);
+            if (BIASED) off2 = f2_add(off2, step2);
           }
           float a0, a1, b0, b1;
           f2_unpack(acc0, a0, a1);
           f2_unpack(acc1, b0, b1);
           sum = (a0 + a1) + (b0 + b1);
-        };
-        if (j == 0 && u == 0) m = maximum();
-        probabilities();
-        const bool grown = live && any && (!(sum <= 1099511627776.0f) || m == -INFINITY);
-        if (__any_sync(0xFFFFFFFFu, grown) && (j > 0 || u > 0)) {
-          // some row of the warp outgrew its reference: find the unit's maxima, bring O and l to the new references and
-          // take the probabilities again. O must be at rest: the products of the unit before this one are done once
-          // S(j) is (u = 0) or once pva_done says so (u = 1).
-          const float m_new = fmaxf(m, maximum());
-          const float f = m == -INFINITY || m_new == -INFINITY ? 0.0f : paged_ex2(m - m_new);
-          if (u == 1 && !mbar_wait(pva_done(t), j & 1u, abort_smem, tflag, 38)) { ok = false; break; }
-          fence_after_sync();
-#pragma unroll 1
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t v[32];
-            tmem_ld_x32(t_o + c * 32, v);
+          done = done && !__any_sync(0xFFFFFFFFu, live && !(sum <= 1099511627776.0f));
+        }
+        if (!done) {
+          // The general form: masks, and the move of the references. Scores in units of log2 are taken from tensor memory
+          // again, 32 at a time.
+          auto scores = [&](int h, float* x) {
+            uint32_t sr[32];
+            tmem_ld_x32(t_s + 64 * u + 32 * h, sr);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = m_new == m ? v[i] : __float_as_uint(__uint_as_float(v[i]) * f);
-            tmem_st_x32(t_o + c * 32, v);
+            for (int i = 0; i < 32; ++i) {
+              const int k = 32 * h + i;
+              float y = __uint_as_float(sr[i]);
+              y = (CAPPED ? paged_tanh(y * p.inv_cap) : y) * mult;
+              if (BIASED) y = fmaf(-slope, fabsf(float(qpos - kabs - k)), y);
+              x[i] = (k < vis && k >= first) || k < pre ? y : -INFINITY;
+            }
+          };
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
+            scores(h, x);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
           }
-          tmem_st_wait();
-          if (m_new != m) l *= f;
+          // a reference moves where it is not there yet, or 2^20 and more behind (short of what sends a unit here)
+          const float m_new = mx > m + 20.0f ? mx : m;
+          if (!begin && __any_sync(0xFFFFFFFFu, m_new != m)) {
+            // O must be at rest: the products of the unit before this one are done once S(j) is (u = 0) or once pva_done
+            // says so (u = 1)
+            const float f = m == -INFINITY ? 0.0f : paged_ex2(m - m_new);
+            if (u == 1 && !mbar_wait(pva_done(t), j & 1u, abort_smem, tflag, 38)) { ok = false; break; }
+            fence_after_sync();
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t v[32];
+              tmem_ld_x32(t_o + c * 32, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = m_new == m ? v[i] : __float_as_uint(__uint_as_float(v[i]) * f);
+              tmem_st_x32(t_o + c * 32, v);
+            }
+            tmem_st_wait();
+            if (m_new != m) l *= f;
+          }
           m = m_new;
-          probabilities();
+          const float off = m == -INFINITY ? 0.0f : m;
+          sum = 0.0f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[32];
+            scores(h, x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float p0 = paged_ex2(x[2 * i] - off), p1 = paged_ex2(x[2 * i + 1] - off);
+              sum += p0 + p1;
+              w[16 * h + i] = pack2(p0, p1);
+            }
+          }
         }
         tmem_st_x32(t_s + 64 * u, w);
         tmem_st_wait();
@@ -661,14 +709,15 @@ paged_prompt_join_kernel(const __grid_constant__ PromptParams p) {
   }
 }
 
-template <int D, bool FP4>
-int launch_prompt(mb_ctx* ctx, cudaStream_t stream, const PromptParams& p, uint32_t once_bit) {
+template <int D, bool FP4, bool CAPPED, bool BIASED>
+int launch_prompt(mb_ctx* ctx, cudaStream_t stream, const PromptParams& p) {
   using Shape = PromptShape<D, FP4>;
+  constexpr uint32_t once_bit = 1u << (8 + (D == 128) + 2 * FP4 + 4 * CAPPED + 8 * BIASED);
   if (!(ctx->paged_once.load(std::memory_order_acquire) & once_bit)) {
-    MB_CUDA_OK(ctx, cudaFuncSetAttribute(paged_prompt_kernel<D, FP4>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+    MB_CUDA_OK(ctx, cudaFuncSetAttribute(paged_prompt_kernel<D, FP4, CAPPED, BIASED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
     ctx->paged_once.fetch_or(once_bit, std::memory_order_release);
   }
-  MB_CUDA_OK(ctx, mb_launch_pdl(paged_prompt_kernel<D, FP4>, dim3(p.blocks * p.c.kv_heads, p.splits), dim3(Shape::THREADS),
+  MB_CUDA_OK(ctx, mb_launch_pdl(paged_prompt_kernel<D, FP4, CAPPED, BIASED>, dim3(p.blocks * p.c.kv_heads, p.splits), dim3(Shape::THREADS),
                                 Shape::SMEM, stream, p));
   if (p.splits > 1)
     MB_CUDA_OK(ctx, mb_launch_pdl(paged_prompt_join_kernel<D>, dim3(p.blocks * p.c.kv_heads, 8), dim3(256), 0, stream, p));
@@ -746,8 +795,13 @@ MB_API int mb_paged_prompt(mb_ctx* ctx, mb_stream stream_, const void* q, size_t
     memset(&p.tmap_k, 0, sizeof p.tmap_k);
     memset(&p.tmap_v, 0, sizeof p.tmap_v);
   }
-  if (kv->d == 128) rc = fp4 ? launch_prompt<128, true>(ctx, stream, p, 1u << 8) : launch_prompt<128, false>(ctx, stream, p, 1u << 9);
-  else rc = fp4 ? launch_prompt<64, true>(ctx, stream, p, 1u << 10) : launch_prompt<64, false>(ctx, stream, p, 1u << 11);
+  const bool cap = terms->softcap > 0.0f, bias = terms->slopes != nullptr;
+#define MB_PROMPT(DD, F) \
+  rc = cap ? (bias ? launch_prompt<DD, F, true, true>(ctx, stream, p) : launch_prompt<DD, F, true, false>(ctx, stream, p)) \
+           : (bias ? launch_prompt<DD, F, false, true>(ctx, stream, p) : launch_prompt<DD, F, false, false>(ctx, stream, p))
+  if (kv->d == 128) { if (fp4) MB_PROMPT(128, true); else MB_PROMPT(128, false); }
+  else { if (fp4) MB_PROMPT(64, true); else MB_PROMPT(64, false); }
+#undef MB_PROMPT
   if (rc) return rc;
   MB_LAUNCH_OK(ctx);
   return MB_OK;
