@@ -496,6 +496,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
     const float mult = CAPPED ? p.cap_log2 : p.scale_log2;
     const float slope = BIASED && mine ? __ldg(p.slopes + kvh * p.group + hg) * 1.4426950408889634f : 0.0f;
     const int window = p.c.window ? int(p.c.window) : 0x40000000;
+    const bool idle = !__any_sync(0xFFFFFFFFu, live);           // no row of the warp has a query: its P may stay what it is
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (uint32_t j = 0; ok && j < n_tiles; ++j) {
@@ -514,7 +515,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
         float sum = 0.0f;
         // The ordinary unit: every key seen by every row of the warp (what rows without a query hold does not matter),
         // references at hand.
-        bool done = !begin && __all_sync(0xFFFFFFFFu, !live || (m > -INFINITY && ((vis >= 64 && first <= 0) || (pre >= 64 && (!BIASED || qpos >= kabs + 63)))));
+        bool done = !begin && !idle && __all_sync(0xFFFFFFFFu, !live || (m > -INFINITY && ((vis >= 64 && first <= 0) || (pre >= 64 && (!BIASED || qpos >= kabs + 63)))));
         if (done) {
           uint32_t sr[64];
           tmem_ld_x32(t_s + 64 * u, sr);
@@ -557,68 +558,85 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
           sum = (a0 + a1) + (b0 + b1);
           done = done && !__any_sync(0xFFFFFFFFu, live && !(sum <= 1099511627776.0f));
         }
-        if (!done) {
+        if (!done && !idle) {
           // The general form: masks, and the move of the references. Scores in units of log2 are taken from tensor memory
-          // again, 32 at a time.
+          // again, 32 at a time; which of them the row sees is a word of bits.
+          auto bits = [&](int h) -> uint32_t {
+            auto below = [](int n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+            return (below(vis - 32 * h) & ~below(first - 32 * h)) | below(pre - 32 * h);
+          };
           auto scores = [&](int h, float* x) {
             uint32_t sr[32];
             tmem_ld_x32(t_s + 64 * u + 32 * h, sr);
             tmem_ld_wait();
+            const uint32_t seen = bits(h);
+            const float away = float(qpos - kabs - 32 * h);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const int k = 32 * h + i;
               float y = __uint_as_float(sr[i]);
               y = (CAPPED ? paged_tanh(y * p.inv_cap) : y) * mult;
-              if (BIASED) y = fmaf(-slope, fabsf(float(qpos - kabs - k)), y);
-              x[i] = (k < vis && k >= first) || k < pre ? y : -INFINITY;
+              if (BIASED) y = fmaf(-slope, fabsf(away - float(i)), y);
+              x[i] = seen & (1u << i) ? y : -INFINITY;
             }
           };
-          float mx = -INFINITY;
+          // a row that sees its first keys needs a reference
+          bool move = __any_sync(0xFFFFFFFFu, m == -INFINITY && (bits(0) | bits(1)) != 0u);
+          for (;;) {
+            if (move) {
+              float mx = -INFINITY;
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            float x[32];
-            scores(h, x);
+              for (int h = 0; h < 2; ++h) {
+                float x[32];
+                scores(h, x);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
-          }
-          // a reference moves where it is not there yet, or 2^20 and more behind (short of what sends a unit here)
-          const float m_new = mx > m + 20.0f ? mx : m;
-          if (!begin && __any_sync(0xFFFFFFFFu, m_new != m)) {
-            // O must be at rest: the products of the unit before this one are done once S(j) is (u = 0) or once pva_done
-            // says so (u = 1)
-            const float f = m == -INFINITY ? 0.0f : paged_ex2(m - m_new);
-            if (u == 1 && !mbar_wait(pva_done(t), j & 1u, abort_smem, tflag, 38)) { ok = false; break; }
-            fence_after_sync();
+                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, x[i]);
+              }
+              // the other rows' references move where they are 2^20 and more behind
+              const float m_new = mx > m + 20.0f ? mx : m;
+              if (!begin && __any_sync(0xFFFFFFFFu, m_new != m)) {
+                // O must be at rest: the products of the unit before this one are done once S(j) is (u = 0) or once
+                // pva_done says so (u = 1)
+                const float f = m == -INFINITY ? 0.0f : paged_ex2(m - m_new);
+                if (u == 1 && !mbar_wait(pva_done(t), j & 1u, abort_smem, tflag, 38)) { ok = false; break; }
+                fence_after_sync();
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t v[32];
-              tmem_ld_x32(t_o + c * 32, v);
-              tmem_ld_wait();
+                for (int c = 0; c < D / 32; ++c) {
+                  uint32_t v[32];
+                  tmem_ld_x32(t_o + c * 32, v);
+                  tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = m_new == m ? v[i] : __float_as_uint(__uint_as_float(v[i]) * f);
-              tmem_st_x32(t_o + c * 32, v);
+                  for (int i = 0; i < 32; ++i) v[i] = m_new == m ? v[i] : __float_as_uint(__uint_as_float(v[i]) * f);
+                  tmem_st_x32(t_o + c * 32, v);
+                }
+                tmem_st_wait();
+                if (m_new != m) l *= f;
+              }
+              m = m_new;
             }
-            tmem_st_wait();
-            if (m_new != m) l *= f;
-          }
-          m = m_new;
-          const float off = m == -INFINITY ? 0.0f : m;
-          sum = 0.0f;
+            const float off = m == -INFINITY ? 0.0f : m;
+            sum = 0.0f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float x[32];
-            scores(h, x);
+            for (int h = 0; h < 2; ++h) {
+              float x[32];
+              scores(h, x);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float p0 = paged_ex2(x[2 * i] - off), p1 = paged_ex2(x[2 * i + 1] - off);
-              sum += p0 + p1;
-              w[16 * h + i] = pack2(p0, p1);
+              for (int i = 0; i < 16; ++i) {
+                const float p0 = paged_ex2(x[2 * i] - off), p1 = paged_ex2(x[2 * i + 1] - off);
+                sum += p0 + p1;
+                w[16 * h + i] = pack2(p0, p1);
+              }
             }
+            if (move) break;
+            move = __any_sync(0xFFFFFFFFu, live && !(sum <= 1099511627776.0f));
+            if (!move) break;
           }
+          if (!ok) break;
         }
-        tmem_st_x32(t_s + 64 * u, w);
-        tmem_st_wait();
-        l += sum;
+        if (!idle) {
+          tmem_st_x32(t_s + 64 * u, w);
+          tmem_st_wait();
+          l += sum;
+        }
         fence_before_sync();
         mbar_arrive(p_full(t, u));
       }
