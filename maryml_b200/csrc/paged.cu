@@ -289,7 +289,7 @@ MB_API int mb_paged_append(mb_ctx* ctx, mb_stream stream_, const void* qkv, size
   AppendParams p;
   int rc = paged_view(ctx, "paged_append", kv, nullptr, kv ? kv->kv_heads : 1, &p.c);
   if (rc) return rc;
-  MB_REQUIRE(ctx, qkv && q_out && inv_freq, "paged_append: null argument");
+  MB_REQUIRE(ctx, inv_freq && (tokens == 0 || (qkv && q_out)), "paged_append: null argument");
   MB_REQUIRE(ctx, hq > 0 && hq <= 65535, "paged_append: bad query head count %zu", hq);
   const size_t heads = hq + 2 * kv->kv_heads;
   MB_REQUIRE(ctx, qkv_stride >= heads * kv->d && qkv_stride % 8 == 0,

@@ -776,7 +776,7 @@ MB_API int mb_paged_prompt(mb_ctx* ctx, mb_stream stream_, const void* q, size_t
   MB_REQUIRE(ctx, ctx && terms, "paged_prompt: null argument");
   int rc = paged_view(ctx, "paged_prompt", kv, terms, heads, &p.c);
   if (rc) return rc;
-  MB_REQUIRE(ctx, q && out && cu_q && mb_aligned(cu_q, 4) && mb_aligned(q, 16) && mb_aligned(out, 16),
+  MB_REQUIRE(ctx, cu_q && (tokens == 0 || (q && out)) && mb_aligned(cu_q, 4) && mb_aligned(q, 16) && mb_aligned(out, 16),
              "paged_prompt: null argument, or q and out without 16-byte alignment");
   MB_REQUIRE(ctx, heads / kv->kv_heads <= QT, "paged_prompt: at most %d query heads per KV head, got %zu", QT, heads / kv->kv_heads);
   if (tokens == 0) return MB_OK;

@@ -16,7 +16,11 @@ import torch
 
 from . import _lib
 from ._lib import MaryError, lib, context
-from .nvfp4 import _p, _stream
+
+# A decode step calls these functions once per layer: the checks below are written to cost a microsecond or two, and the
+# current stream is asked for without building a Stream object.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_bf16_t, _i32_t, _u8_t, _f32_t = torch.bfloat16, torch.int32, torch.uint8, torch.float32
 
 
 def _refuse(text):
@@ -24,10 +28,14 @@ def _refuse(text):
 
 
 def _int32(t, name, dims, dev):
-    if t.dtype != torch.int32 or t.dim() != dims or t.device != dev:
+    if t.dtype is not _i32_t or t.dim() != dims or t.device != dev:
         _refuse(f"{name} is a {dims}-d int32 tensor on {dev}, not {tuple(t.shape)} {t.dtype} on {t.device}")
-    if t.numel() and t.stride(-1) != 1:
+    if t.stride(dims - 1) != 1 and t.shape[-1] > 1:
         _refuse(f"{name} is read with unit stride in its last dimension, not {t.stride()}")
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
 
 
 class PagedCache:
@@ -37,30 +45,32 @@ class PagedCache:
     multiple of 16. The tensors are used as they are, nothing is copied."""
 
     def __init__(self, k, v, k_scales=None, v_scales=None, head_dim=None):
-        planes = [t for t in (k, v, k_scales, v_scales) if t is not None]
-        for t in planes:
-            if not (t.is_cuda and t.is_contiguous() and t.device == k.device):
-                _refuse("page pools are contiguous tensors on one CUDA device")
-        if k.shape != v.shape or k.dtype != v.dtype:
+        dev = k.device
+        if not (k.is_cuda and k.is_contiguous() and v.is_contiguous() and v.device == dev):
+            _refuse("page pools are contiguous tensors on one CUDA device")
+        if k.shape != v.shape or k.dtype is not v.dtype:
             _refuse(f"k and v pools differ: {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
         if k_scales is None and v_scales is None:
-            if k.dtype != torch.bfloat16 or k.dim() != 4:
+            if k.dtype is not _bf16_t or k.dim() != 4:
                 _refuse(f"a pool without scales is [pages, page_size, kv_heads, head_dim] bf16, not {tuple(k.shape)} {k.dtype}")
-            if head_dim is not None and head_dim != k.shape[3]:
-                _refuse(f"the pool's head_dim is {k.shape[3]}, not {head_dim}")
-            self.elem, self.kv_heads, self.head_dim = _lib.KV_BF16, k.shape[2], k.shape[3]
+            self.pages, self.page_size, self.kv_heads, self.head_dim = k.shape
+            if head_dim is not None and head_dim != self.head_dim:
+                _refuse(f"the pool's head_dim is {self.head_dim}, not {head_dim}")
+            self.elem = _lib.KV_BF16
         else:
             if head_dim is None or k_scales is None or v_scales is None:
                 _refuse("an NVFP4 pool takes both scale planes and head_dim")
             if k.dtype != torch.uint8 or k.dim() != 3 or head_dim <= 0 or (2 * k.shape[2]) % head_dim:
                 _refuse(f"NVFP4 codes are [pages, page_size, kv_heads * {head_dim} / 2] uint8, not {tuple(k.shape)} {k.dtype}")
             for t in (k_scales, v_scales):
-                if t.dtype != torch.uint8 or tuple(t.shape) != (k.shape[0], k.shape[1], k.shape[2] // 8):
+                if not t.is_contiguous() or t.device != dev:
+                    _refuse("page pools are contiguous tensors on one CUDA device")
+                if t.dtype is not _u8_t or tuple(t.shape) != (k.shape[0], k.shape[1], k.shape[2] // 8):
                     _refuse(f"NVFP4 scales of this pool are {(k.shape[0], k.shape[1], k.shape[2] // 8)} uint8, not "
                             f"{tuple(t.shape)} {t.dtype}")
-            self.elem, self.kv_heads, self.head_dim = _lib.KV_NVFP4, 2 * k.shape[2] // head_dim, head_dim
-        self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
-        self.pages, self.page_size, self.device = k.shape[0], k.shape[1], k.device
+            self.pages, self.page_size, width = k.shape
+            self.elem, self.kv_heads, self.head_dim = _lib.KV_NVFP4, 2 * width // head_dim, head_dim
+        self.k, self.v, self.k_scales, self.v_scales, self.device = k, v, k_scales, v_scales, dev
 
     @classmethod
     def empty(cls, pages, page_size, kv_heads, head_dim, nvfp4=False, device=None):
@@ -80,14 +90,13 @@ class PagedCache:
         batch, width = block_table.shape
         if lens.shape[0] != batch:
             _refuse(f"block_table has {batch} rows, lens {lens.shape[0]} entries")
-        return _lib.PagedKv(self.k.data_ptr(), self.v.data_ptr(), self.k_scales.data_ptr() if self.k_scales is not None else None,
-                            self.v_scales.data_ptr() if self.v_scales is not None else None, self.elem, self.pages,
+        return _lib.PagedKv(self.k.data_ptr(), self.v.data_ptr(), _ptr(self.k_scales), _ptr(self.v_scales), self.elem, self.pages,
                             self.page_size, self.kv_heads, self.head_dim, block_table.data_ptr(), width,
                             block_table.stride(0) if batch > 1 else max(width, 1), lens.data_ptr(), batch)
 
 
 def _terms(cache, batch, heads, scale, softcap, window, slopes, prefix):
-    if slopes is not None and (slopes.dtype != torch.float32 or slopes.shape != (heads,) or not slopes.is_contiguous()
+    if slopes is not None and (slopes.dtype is not _f32_t or slopes.shape != (heads,) or not slopes.is_contiguous()
                                or slopes.device != cache.device):
         _refuse(f"slopes is a contiguous f32 tensor of {heads} heads on {cache.device}")
     if prefix is not None:
@@ -96,13 +105,12 @@ def _terms(cache, batch, heads, scale, softcap, window, slopes, prefix):
             _refuse(f"prefix has {prefix.shape[0]} entries for {batch} sequences")
     if window < 0:
         _refuse(f"window is 0 (none) or a positive number of rows, not {window}")
-    return _lib.ScoreTerms(float(scale) if scale is not None else 1.0 / math.sqrt(cache.head_dim), float(softcap), int(window),
-                           slopes.data_ptr() if slopes is not None else None,
-                           prefix.data_ptr() if prefix is not None else None)
+    return _lib.ScoreTerms(scale if scale is not None else 1.0 / math.sqrt(cache.head_dim), softcap, window, _ptr(slopes),
+                           _ptr(prefix))
 
 
 def _bf16(t, name, dev):
-    if t.dtype != torch.bfloat16 or t.device != dev or not t.is_contiguous():
+    if t.dtype is not _bf16_t or t.device != dev or not t.is_contiguous():
         _refuse(f"{name} is a contiguous bf16 tensor on {dev}")
 
 
@@ -118,7 +126,7 @@ def _out_like(q, out):
 def _workspace(workspace, need, dev):
     if need and (workspace is None or workspace.device != dev or workspace.numel() * workspace.element_size() < need
                  or workspace.data_ptr() % 256 or not workspace.is_contiguous()):
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+        workspace = torch.empty(need, dtype=_u8_t, device=dev)
     return workspace
 
 
@@ -131,13 +139,13 @@ def paged_append(qkv, cache, block_table, lens, inv_freq, cu_q=None, positions=N
     [tokens, hq, head_dim]; rows at or past cu_q[batch] stay as they are in `out`."""
     dev, d = cache.device, cache.head_dim
     kv = cache._kv(block_table, lens)
-    if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.device != dev or (qkv.numel() and qkv.stride(1) != 1):
+    if qkv.dtype is not _bf16_t or qkv.dim() != 2 or qkv.device != dev or qkv.stride(1) != 1:
         _refuse(f"qkv is a 2-d bf16 tensor on {dev} with unit stride along its rows")
     tokens, width = qkv.shape
     hq = width // d - 2 * cache.kv_heads
     if width % d or hq <= 0:
         _refuse(f"a row of {width} values is not (hq + 2 * {cache.kv_heads}) heads of {d}")
-    if inv_freq.dtype != torch.float32 or inv_freq.numel() != d // 2 or not inv_freq.is_contiguous() or inv_freq.device != dev:
+    if inv_freq.dtype is not _f32_t or inv_freq.numel() != d // 2 or not inv_freq.is_contiguous() or inv_freq.device != dev:
         _refuse(f"inv_freq is {d // 2} contiguous f32 values on {dev}")
     if cu_q is not None:
         _int32(cu_q, "cu_q", 1, dev)
@@ -158,14 +166,15 @@ def paged_append(qkv, cache, block_table, lens, inv_freq, cu_q=None, positions=N
     elif sections is not None:
         _refuse("sections belong to positions")
     if out is None:
-        out = torch.empty((tokens, hq, d), dtype=torch.bfloat16, device=dev)
+        out = torch.empty((tokens, hq, d), dtype=_bf16_t, device=dev)
     else:
         _bf16(out, "out", dev)
         if out.numel() != tokens * hq * d:
             _refuse(f"out is [{tokens}, {hq}, {d}], not {tuple(out.shape)}")
     ctx = context(dev.index)
-    ctx.check(lib.mb_paged_append(ctx.handle, _stream(), _p(qkv), qkv.stride(0) if tokens > 1 else width, tokens, hq,
-                                  C.byref(kv), _p(cu_q), _p(inv_freq), _p(positions), axes, ends, _p(out)))
+    ctx.check(lib.mb_paged_append(ctx.handle, _raw_stream(dev.index), qkv.data_ptr(), qkv.stride(0) if tokens > 1 else width,
+                                  tokens, hq, C.byref(kv), _ptr(cu_q), inv_freq.data_ptr(), _ptr(positions), axes, ends,
+                                  out.data_ptr()))
     return out
 
 
@@ -187,8 +196,8 @@ def paged_attention_decode(q, cache, block_table, lens, scale=None, softcap=0.0,
     ctx = context(cache.device.index)
     need = lib.mb_paged_decode_workspace(ctx.handle, C.byref(kv), nq, heads)
     workspace = _workspace(workspace, need, cache.device)
-    ctx.check(lib.mb_paged_decode(ctx.handle, _stream(), _p(q), nq, heads, C.byref(kv), C.byref(terms), _p(out), _p(workspace),
-                                  workspace.numel() * workspace.element_size() if need else 0))
+    ctx.check(lib.mb_paged_decode(ctx.handle, _raw_stream(ctx.device), q.data_ptr(), nq, heads, C.byref(kv), C.byref(terms),
+                                  out.data_ptr(), _ptr(workspace), need))
     return out
 
 
@@ -211,7 +220,6 @@ def paged_attention_prompt(q, cu_q, cache, block_table, lens, scale=None, softca
     ctx = context(cache.device.index)
     need = lib.mb_paged_prompt_workspace(ctx.handle, C.byref(kv), tokens, heads)
     workspace = _workspace(workspace, need, cache.device)
-    ctx.check(lib.mb_paged_prompt(ctx.handle, _stream(), _p(q), tokens, heads, C.byref(kv), _p(cu_q), C.byref(terms), _p(out),
-                                  _p(workspace) if need else None,
-                                  workspace.numel() * workspace.element_size() if need else 0))
+    ctx.check(lib.mb_paged_prompt(ctx.handle, _raw_stream(ctx.device), q.data_ptr(), tokens, heads, C.byref(kv), cu_q.data_ptr(),
+                                  C.byref(terms), out.data_ptr(), _ptr(workspace) if need else None, need))
     return out
