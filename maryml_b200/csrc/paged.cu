@@ -178,7 +178,7 @@ paged_append_kernel(const __grid_constant__ AppendParams p) {
         dst[g] = r0;
         dst[G + g] = r1;
       }
-    } else {
+    } else if (__any_sync(0xFFFFFFFFu, head >= p.hq)) {      // query heads have nothing to quantize
       uint32_t s0, s1;
       const uint32_t c0 = quant_half_recip(r0, s0), c1 = quant_half_recip(r1, s1);
       if (head >= p.hq && at >= 0) {

@@ -18,6 +18,7 @@ from . import _lib
 from ._lib import lib, context, MaryError
 from . import nvfp4 as nv
 from .attention import flash_attention
+from .paged import paged_append, paged_attention_decode, paged_attention_prompt
 
 _p = nv._p
 _stream = nv._stream
@@ -452,10 +453,17 @@ class DecoderLayer:
         residual add folded into the next norm. Every value is computed by the arithmetic of the
         separate kernels. `before_rope` / `after_rope` are hooks of the chunked prompt path."""
         rows = x.shape[0]
+        if self.fused is None or rows > self.fused.t_max:
+            if self._rows_shard(rows):
+                return self._forward_rows_sharded(x, batch, past, k_cache, v_cache, out, after_rope, before_rope)
+        return self._after_attention(x, self._attention(x, batch, past, k_cache, v_cache, after_rope, before_rope), out)
+
+    def _after_attention(self, x, a, out=None):
+        """The layer from the attention's output a [rows, local_heads * D] on."""
+        rows = x.shape[0]
         if self.fused is not None and rows <= self.fused.t_max:
             # peer-memory exchange: the row-parallel products scatter their partial tiles, one kernel per
             # exchange reduces, adds the residual and gathers
-            a = self._attention(x, batch, past, k_cache, v_cache, after_rope, before_rope)
             residual = self._reduced_residual(x, a, self.wo)
             _, nq_ = self._norm_quantize(residual, None, self.post_gain)
             act = nv.gemm_w4a4_stacked(nq_[0], nq_[1], self.wgu, nq_[2],
@@ -465,9 +473,7 @@ class DecoderLayer:
                 out.copy_(y)
                 return out
             return y
-        if self._rows_shard(rows):
-            return self._forward_rows_sharded(x, batch, past, k_cache, v_cache, out, after_rope, before_rope)
-        o_sum = self._all_reduce(self.half_attention(x, batch, past, k_cache, v_cache, after_rope, before_rope))
+        o_sum = self._all_reduce(self._linear(a, self.wo, out_dtype=torch.float32))
         if not (self.group is not None and self.tp.is_split()):
             # nothing to sum across ranks: the down product hands over bf16 (half the bytes written and read back),
             # bf16(residual + bf16(down)) either way
@@ -475,6 +481,25 @@ class DecoderLayer:
             return add(residual, down, out=out)
         residual, down = self.half_mlp(x, o_sum)
         return self.finish(residual, self._all_reduce(down), out=out)
+
+    def forward_paged(self, x, cache, block_table, lens, cu_q=None, **terms):
+        """The layer over a paged cache (`paged.PagedCache` of this rank's KV heads) for a continuous batch: x [tokens,
+        hidden] bf16 holds the new tokens of every sequence, which lens [batch] already counts. Without cu_q every sequence
+        has the same number of them (a decode step: one); with cu_q [batch + 1] they are ragged (prompts and chunks).
+        terms: softcap, window, slopes, prefix of the attention. All lengths are read on the device: a captured step is
+        replayed as the batch grows. The rotation is paged_append's, rounded once (forward keeps the rounding points of the
+        reference's tables, src/models/breeze/cuda_ops.rs:286-320). Built with fuse=True."""
+        if not self.fuse:
+            raise ValueError("forward_paged needs the stacked projections (fuse=True)")
+        batch, D = block_table.shape[0], self.cfg.head_dim
+        _, xq = self._norm_quantize(x, None, self.input_gain)
+        qkv = nv.gemm_w4a4_stacked(xq[0], xq[1], self.wqkv, xq[2])
+        q = paged_append(qkv, cache, block_table, lens, self.inv_freq, cu_q=cu_q)
+        if cu_q is None:
+            a = paged_attention_decode(q.view(batch, -1, self.local_heads, D), cache, block_table, lens, **terms)
+        else:
+            a = paged_attention_prompt(q, cu_q, cache, block_table, lens, **terms)
+        return self._after_attention(x, a.view(x.shape[0], self.local_heads * D))
 
     # Prompts of at least this many rows per rank keep their rows sharded between the two exchanges
     # (MB_TP_ROW_SHARD=0 in the environment keeps the plain all-reduce, for comparison runs).

@@ -438,3 +438,271 @@ def test_bad_entries_are_contained_and_flagged(pg, nvfp4):
     rc, flags = pg.context(0).check_flags()
     assert rc != 0 and flags[2] in (1, 2, 3)
     assert all(torch.equal(t, u) for t, u in zip(planes, before))
+
+
+# ---- the operators together, as a server uses them ---------------------------------------------------
+def test_serving_run_with_a_replayed_step(pg):
+    """Ragged prompts in two chunks, then decode steps replayed from one captured graph while lengths and tables grow on the
+    device; every attention output against the plain form on the rows the cache then holds."""
+    hq, kvh, d, page, batch = 8, 2, 128, 16, 3
+    chunks = [[37, 100, 5], [20, 61, 0]]
+    steps = 20
+    ends = [sum(c[b] for c in chunks) + steps for b in range(batch)]
+    s = Setup(pg, ends, page, kvh, d, seed=21)
+    full_table = s.table.clone()
+    f = inv_freq_of(d)
+    heads = hq + 2 * kvh
+    done = [0] * batch
+    for c in chunks:
+        qkv = torch.randn((sum(c), heads * d), device="cuda", generator=s.gen).to(torch.bfloat16)
+        cu = torch.tensor([0] + list(np.cumsum(c)), dtype=torch.int32, device="cuda")
+        done = [a + n for a, n in zip(done, c)]
+        lens = torch.tensor(done, dtype=torch.int32, device="cuda")
+        q = pg.paged_append(qkv, s.cache, s.table, lens, f, cu_q=cu)
+        out = pg.paged_attention_prompt(q, cu, s.cache, s.table, lens, window=70)
+        s.lens_host = list(done)
+        t0 = 0
+        for b, n in enumerate(c):
+            pos = torch.arange(done[b] - n, done[b], device="cuda")
+            o, a = plain_attention(q[t0:t0 + n].double(), s.rows(b, "k"), s.rows(b, "v"), pos, 1.0 / math.sqrt(d), window=70)
+            check_attention(out[t0:t0 + n], o, a)
+            t0 += n
+    # a step on static buffers: lengths and table are rewritten between replays (pages appear as they are needed)
+    lens = torch.tensor(done, dtype=torch.int32, device="cuda")
+    table = torch.full_like(full_table, -1)
+    qkv = torch.zeros((batch, heads * d), dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.Stream()
+
+    def step():
+        lens.add_(1)
+        q = pg.paged_append(qkv, s.cache, table, lens, f)
+        return q, pg.paged_attention_decode(q.view(batch, 1, hq, d), s.cache, table, lens, window=70)
+
+    def fill(upto):
+        for b, n in enumerate(upto):
+            table[b, :-(-n // page)] = full_table[b, :-(-n // page)]
+
+    fill([n + 1 for n in done])
+    with torch.cuda.stream(stream):
+        stream.wait_stream(torch.cuda.default_stream())
+        step()                                             # warm-up: this row is written again by the first replay
+        lens.sub_(1)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        q, out = step()
+    for i in range(steps):
+        fill([n + 1 for n in done])
+        qkv.copy_(torch.randn((batch, heads * d), device="cuda", generator=s.gen))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        done = [n + 1 for n in done]
+        assert lens.tolist() == done
+        s.lens_host = list(done)
+        for b in range(batch):
+            at = int(full_table[b, (done[b] - 1) // page]) * page + (done[b] - 1) % page
+            assert torch.equal(s.cache.v.view(-1, kvh, d)[at], qkv.view(batch, heads, d)[b, hq + kvh:])
+            o, a = plain_attention(q[b:b + 1].double(), s.rows(b, "k"), s.rows(b, "v"), torch.tensor([done[b] - 1], device="cuda"),
+                                   1.0 / math.sqrt(d), window=70)
+            check_attention(out[b], o, a)
+    no_flags(pg)
+
+
+def test_layer_over_a_paged_cache(pg):
+    """forward_paged is its parts in order, bit for bit; and its first layer of arithmetic is forward's: the rows it appends
+    are the contiguous cache's up to the rounding points of the rotation."""
+    from maryml_b200 import layer, nvfp4 as nv
+    cfg = layer.LayerConfig(hidden=512, heads=4, kv_heads=2, head_dim=128, inter=1024)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    full = {}
+    for name, n, k in (("q", 512, 512), ("k", 256, 512), ("v", 256, 512), ("o", 512, 512), ("gate", 1024, 512), ("up", 1024, 512),
+                       ("down", 512, 1024)):
+        w = (torch.randn((n, k), device="cuda", generator=g) * 0.02).to(torch.bfloat16)
+        p = nv.Nvfp4.quantize(w)
+        full[name] = (p.codes, p.scales, p.scale2)
+    gain = torch.ones(512, dtype=torch.bfloat16, device="cuda")
+    L = layer.DecoderLayer(cfg, full, gain, gain)
+    q_len = [70, 33]
+    lens = [70, 50]
+    s = Setup(pg, lens, 16, 2, 128, seed=31)
+    x = torch.randn((sum(q_len), 512), device="cuda", generator=g).to(torch.bfloat16)
+    cu = torch.tensor([0, 70, 103], dtype=torch.int32, device="cuda")
+    y = L.forward_paged(x, s.cache, s.table, s.lens, cu_q=cu, softcap=30.0)
+    _, xq = L._norm_quantize(x, None, L.input_gain)
+    qkv = nv.gemm_w4a4_stacked(xq[0], xq[1], L.wqkv, xq[2])
+    q = pg.paged_append(qkv, s.cache, s.table, s.lens, L.inv_freq, cu_q=cu)
+    a = pg.paged_attention_prompt(q, cu, s.cache, s.table, s.lens, softcap=30.0)
+    o_sum = L._linear(a.reshape(103, 512), L.wo, out_dtype=torch.float32)
+    residual, down = L.half_mlp(x, o_sum, down_dtype=torch.bfloat16)
+    assert torch.equal(y, layer.add(residual, down))
+    # the contiguous layer's rows of the fresh sequence
+    kc, vc = (torch.zeros((1, 70, 2, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    L.forward(x[:70], 1, 0, kc, vc)
+    assert torch.equal(s.rows(0, "v"), vc[0].double())
+    # forward rounds cos and sin to bf16 (2^-8 of each), both products and the sum: 2^-8 * 3 of |x| + |y|, and paged_append's one
+    size = (kc[0].double()[..., :64].abs() + kc[0].double()[..., 64:].abs()).repeat(1, 1, 2) * math.sqrt(2.0)
+    assert ((s.rows(0, "k") - kc[0].double()).abs() <= 4 * 2.0 ** -8 * size).all()
+    # a decode step of one token each
+    s.lens.add_(0)
+    y1 = L.forward_paged(x[:2], s.cache, s.table, s.lens)
+    q = pg.paged_append(nv.gemm_w4a4_stacked(*L._quantize(layer.rmsnorm(x[:2], L.input_gain, cfg.eps))[:2], L.wqkv, 2), s.cache,
+                        s.table, s.lens, L.inv_freq)
+    a = pg.paged_attention_decode(q.view(2, 1, 4, 128), s.cache, s.table, s.lens)
+    residual, down = L.half_mlp(x[:2], L._linear(a.view(2, 512), L.wo, out_dtype=torch.float32), down_dtype=torch.bfloat16)
+    assert torch.equal(y1, layer.add(residual, down))
+    with pytest.raises(ValueError):
+        layer.DecoderLayer(cfg, full, gain, gain, fuse=False).forward_paged(x, s.cache, s.table, s.lens, cu_q=cu)
+    no_flags(pg)
+
+
+def test_another_stream_and_overlapping_calls(pg):
+    """Two streams at once, each with its own workspace from the allocator: both as alone."""
+    setups = [Setup(pg, [3000 + 7 * i, 40, 900], 64, 2, 128, seed=40 + i) for i in range(2)]
+    qs = [torch.randn((3, 1, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16) for s in setups]
+    qp = [torch.randn((130, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16) for s in setups]
+    cu = torch.tensor([0, 90, 130, 130], dtype=torch.int32, device="cuda")
+    want = [(pg.paged_attention_decode(q, s.cache, s.table, s.lens), pg.paged_attention_prompt(p, cu, s.cache, s.table, s.lens))
+            for s, q, p in zip(setups, qs, qp)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                s = setups[i]
+                got[i].append((pg.paged_attention_decode(qs[i], s.cache, s.table, s.lens),
+                               pg.paged_attention_prompt(qp[i], cu, s.cache, s.table, s.lens)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, b in got[i]:
+            assert torch.equal(a, want[i][0]) and torch.equal(b, want[i][1])
+    no_flags(pg)
+
+
+def test_strided_tables_and_kept_workspace(pg):
+    s = Setup(pg, [500, 77], 16, 2, 128, seed=50)
+    wide = torch.full((2, s.table.shape[1] + 9), 1 << 29, dtype=torch.int32, device="cuda")
+    wide[:, 4:4 + s.table.shape[1]] = s.table
+    view = wide[:, 4:4 + s.table.shape[1]]
+    q = torch.randn((2, 1, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16)
+    want = pg.paged_attention_decode(q, s.cache, s.table, s.lens)
+    ws = torch.full((64 << 20,), 0xFF, dtype=torch.uint8, device="cuda")          # its contents do not matter
+    out = torch.empty_like(q)
+    for _ in range(3):
+        assert pg.paged_attention_decode(q, s.cache, view, s.lens, out=out, workspace=ws) is out
+        assert torch.equal(out, want)
+    no_flags(pg)
+
+
+def test_an_sm_limit_changes_the_cut_not_the_result(pg):
+    from maryml_b200 import _lib
+    s = Setup(pg, [9000, 100], 64, 2, 128, seed=51)
+    q = torch.randn((2, 1, 8, 128), device="cuda", generator=s.gen).to(torch.bfloat16)
+    a = pg.paged_attention_decode(q, s.cache, s.table, s.lens)
+    ctx = pg.context(0)
+    ctx.check(_lib.lib.mb_ctx_set_sm_limit(ctx.handle, 20))
+    try:
+        b = pg.paged_attention_decode(q, s.cache, s.table, s.lens)
+    finally:
+        ctx.check(_lib.lib.mb_ctx_set_sm_limit(ctx.handle, 0))
+    o, room = plain_attention(q[0].double(), s.rows(0, "k"), s.rows(0, "v"), torch.tensor([8999], device="cuda"), 1 / math.sqrt(128))
+    check_attention(a[0], o, room)
+    check_attention(b[0], o, room)
+
+
+def test_a_pool_beyond_two_to_the_32_bytes(pg):
+    """Rows past 2^31 elements and 2^32 bytes of a pool are addressed in 64 bits, by the append and by both readers."""
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB of free device memory")
+    for nvfp4 in (False, True):
+        kvh, d, page = 8, 128, 256
+        pages = (5 << 30) // (page * kvh * d * 2) if not nvfp4 else (5 << 30) // (page * kvh * d // 2)
+        cache = pg.PagedCache.empty(pages, page, kvh, d, nvfp4=nvfp4)
+        n = 300
+        table = torch.tensor([[pages - 1, pages - 3, -1], [1, pages // 2, -1]], dtype=torch.int32, device="cuda")
+        lens = torch.tensor([n, n - 7], dtype=torch.int32, device="cuda")
+        g = torch.Generator(device="cuda").manual_seed(5)
+        hq = 8
+        qkv = torch.randn((2 * n - 7, (hq + 2 * kvh) * d), device="cuda", generator=g).to(torch.bfloat16)
+        cu = torch.tensor([0, n, 2 * n - 7], dtype=torch.int32, device="cuda")
+        q = pg.paged_append(qkv, cache, table, lens, inv_freq_of(d), cu_q=cu)
+        out = pg.paged_attention_prompt(q, cu, cache, table, lens)
+        one = pg.paged_attention_decode(torch.stack((q[n - 1], q[-1])).unsqueeze(1), cache, table, lens)
+        for b, (length, t0) in enumerate(((n, 0), (n - 7, n))):
+            r = torch.arange(length, device="cuda")
+            page_of, row = table[b].long()[r // page], r % page
+            if nvfp4:
+                k, v = (fp4_values(getattr(cache, x)[page_of, row], getattr(cache, x + "_scales")[page_of, row]).view(length, kvh, d)
+                        for x in ("k", "v"))
+            else:
+                k, v = cache.k[page_of, row].double(), cache.v[page_of, row].double()
+                assert torch.equal(cache.v[page_of, row], qkv.view(-1, hq + 2 * kvh, d)[t0:t0 + length, hq + kvh:])
+            o, a = plain_attention(q[t0:t0 + length].double(), k, v, r, 1 / math.sqrt(d))
+            check_attention(out[t0:t0 + length], o, a)
+            check_attention(one[b], o[-1:], a[-1:])
+        del cache
+    no_flags(pg)
+
+
+def test_masked_keys_may_hold_anything(pg):
+    """NaN and infinities in rows nobody sees: behind the length, below a window, in pages of others. Keys a query does not
+    see may be NaN or infinite too (their scores are replaced before they are used)."""
+    for d in (64, 128):
+        s = Setup(pg, [200, 130], 32, 2, d, seed=60)
+        at = lambda b, r: int(s.table[b, r // 32]) * 32 + r % 32
+        k, v = s.cache.k.view(-1, 2, d), s.cache.v.view(-1, 2, d)
+        q = torch.randn((2, 1, 8, d), device="cuda", generator=s.gen).to(torch.bfloat16)
+        want = pg.paged_attention_decode(q, s.cache, s.table, s.lens, window=50).clone()
+        for r in range(0, 150):
+            k[at(0, r)] = float("inf") if r % 2 else float("nan")
+            v[at(0, r)] = float("nan") if r % 2 else float("-inf")
+        assert torch.equal(pg.paged_attention_decode(q, s.cache, s.table, s.lens, window=50), want)
+    no_flags(pg)
+
+
+def test_zero_tokens_are_a_call_that_does_nothing(pg):
+    s = Setup(pg, [5, 6], 16, 2, 128, seed=61)
+    cu = torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = pg.paged_append(torch.empty((0, 12 * 128), dtype=torch.bfloat16, device="cuda"), s.cache, s.table, s.lens, inv_freq_of(128), cu_q=cu)
+    assert q.shape == (0, 8, 128)
+    assert pg.paged_attention_prompt(q, cu, s.cache, s.table, s.lens).shape == (0, 8, 128)
+    no_flags(pg)
+
+
+def test_refusals(pg):
+    from maryml_b200 import MaryError
+    s = Setup(pg, [20, 30], 16, 2, 128, seed=70)
+    q = torch.zeros((2, 1, 8, 128), dtype=torch.bfloat16, device="cuda")
+    qp, cu = q.view(2, 8, 128), torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    qkv = torch.zeros((2, 12 * 128), dtype=torch.bfloat16, device="cuda")
+    f = inv_freq_of(128)
+    dec = lambda **k: pg.paged_attention_decode(k.pop("q", q), k.pop("cache", s.cache), k.pop("t", s.table), k.pop("n", s.lens), **k)
+    pro = lambda **k: pg.paged_attention_prompt(k.pop("q", qp), k.pop("cu", cu), k.pop("cache", s.cache), k.pop("t", s.table), k.pop("n", s.lens), **k)
+    app = lambda **k: pg.paged_append(k.pop("x", qkv), k.pop("cache", s.cache), k.pop("t", s.table), k.pop("n", s.lens), k.pop("f", f), **k)
+    bad_page = pg.PagedCache(*(torch.zeros((4, 24, 2, 128), dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    bad_dim = pg.PagedCache(*(torch.zeros((4, 16, 2, 96), dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    cases = [
+        lambda: dec(q=q.float()), lambda: dec(q=q[:, :, :, :64]), lambda: dec(q=q[:1]), lambda: dec(q=torch.zeros((2, 1, 7, 128), dtype=torch.bfloat16, device="cuda")),
+        lambda: dec(t=s.table.long()), lambda: dec(t=s.table.t()), lambda: dec(t=s.table.cpu()), lambda: dec(n=s.lens[:1]), lambda: dec(n=s.lens.long()),
+        lambda: dec(scale=-1.0), lambda: dec(scale=float("nan")), lambda: dec(scale=0.0), lambda: dec(softcap=-1.0), lambda: dec(softcap=float("inf")),
+        lambda: dec(window=-3), lambda: dec(slopes=torch.zeros(7, device="cuda")), lambda: dec(slopes=torch.zeros(8, dtype=torch.float64, device="cuda")),
+        lambda: dec(prefix=torch.zeros(3, dtype=torch.int32, device="cuda")), lambda: dec(prefix=torch.zeros(2, device="cuda")),
+        lambda: dec(out=torch.zeros((2, 8, 128), dtype=torch.bfloat16, device="cuda")), lambda: dec(cache=bad_page),
+        lambda: dec(cache=bad_dim, q=torch.zeros((2, 1, 8, 96), dtype=torch.bfloat16, device="cuda")), lambda: dec(t=s.table[:, :0]),
+        lambda: pro(q=qp.float()), lambda: pro(q=q), lambda: pro(cu=cu[:2]), lambda: pro(cu=cu.long()), lambda: pro(cu=cu.cpu()),
+        lambda: pro(scale=0.0), lambda: pro(cache=bad_page), lambda: pro(q=torch.zeros((2, 258, 128), dtype=torch.bfloat16, device="cuda")),
+        lambda: app(x=qkv.float()), lambda: app(x=qkv[:, :-1]), lambda: app(x=qkv[:, :4 * 128]), lambda: app(x=qkv.t()), lambda: app(f=f[:32]), lambda: app(f=f.double()),
+        lambda: app(cu_q=cu[:2]), lambda: app(x=torch.zeros((3, 12 * 128), dtype=torch.bfloat16, device="cuda")), lambda: app(sections=(64,)),
+        lambda: app(positions=torch.zeros((3, 2), dtype=torch.int32, device="cuda")), lambda: app(positions=torch.zeros((3, 2), dtype=torch.int32, device="cuda"), sections=(16, 24, 23)),
+        lambda: app(positions=torch.zeros((5, 2), dtype=torch.int32, device="cuda"), sections=(16, 24, 24, 0, 0)), lambda: app(positions=torch.zeros((1, 3), dtype=torch.int32, device="cuda")),
+        lambda: app(x=torch.zeros((2, 12 * 128 + 4), dtype=torch.bfloat16, device="cuda")[:, :12 * 128]), lambda: app(cache=bad_page),
+        lambda: pg.PagedCache(s.cache.k, s.cache.v[:1]), lambda: pg.PagedCache(s.cache.k.float(), s.cache.v.float()),
+        lambda: pg.PagedCache(s.cache.k.transpose(1, 2), s.cache.v.transpose(1, 2)), lambda: pg.PagedCache(s.cache.k, s.cache.v, head_dim=64),
+        lambda: pg.PagedCache(s.cache.k.view(torch.uint8), s.cache.v.view(torch.uint8), s.cache.k, None, head_dim=128),
+    ]
+    for i, c in enumerate(cases):
+        with pytest.raises(MaryError):
+            c()
+            pytest.fail(f"case {i} was not refused")
+    no_flags(pg)
