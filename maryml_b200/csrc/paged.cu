@@ -63,7 +63,9 @@ __global__ void __launch_bounds__(APPEND_THREADS)
 paged_append_kernel(const __grid_constant__ AppendParams p) {
   constexpr int HALF = 8 * G;                        // d / 2
   constexpr int UNITS = APPEND_THREADS / G;          // units of a pass
-  __shared__ float2 turn[TB][HALF];                  // (cos, sin)
+  // (cos, sin) of frequencies 2 i and 2 i + 1 of thread g's eight at [i][g]: the threads of a unit read 16 bytes each, side
+  // by side
+  __shared__ float4 turn[TB][4][G];
   __shared__ long long slot[TB];                     // pool row of a token; -1: nowhere to go, -2: not a token
   __shared__ int row_of[TB];
   mb_grid_dependency_sync();
@@ -135,9 +137,14 @@ paged_append_kernel(const __grid_constant__ AppendParams p) {
     // The angle needs 31 + 24 bits before its multiples of 2 pi are gone; what is left takes 32.
     const double angle = double(pos) * double(__ldg(p.inv_freq + f));
     const double turns = rint(angle * 0.15915494309189535);
+    const double rest = fma(-turns, 6.283185307179586, angle);
+    const float high = float(rest), low = float(rest - double(high));      // low: what f32 rounds off, up to 2^-23
     float s, c;
-    sincosf(float(fma(-turns, 6.283185307179586, angle)), &s, &c);
-    turn[t][f] = make_float2(c, s);
+    sincosf(high, &s, &c);
+    const float s0 = s;
+    s = fmaf(low, c, s);
+    c = fmaf(-low, s0, c);
+    reinterpret_cast<float2*>(&turn[t][(f % 8) / 2][f / 8])[f % 2] = make_float2(c, s);
   }
   __syncthreads();
 
@@ -155,10 +162,12 @@ paged_append_kernel(const __grid_constant__ AppendParams p) {
       unpack8(a, x);
       unpack8(b, y);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 cs = turn[t][g * 8 + j];
+      for (int j = 0; j < 8; j += 2) {
+        const float4 cs = turn[t][j / 2][g];
         o[j] = x[j] * cs.x - y[j] * cs.y;
         w[j] = y[j] * cs.x + x[j] * cs.y;
+        o[j + 1] = x[j + 1] * cs.z - y[j + 1] * cs.w;
+        w[j + 1] = y[j + 1] * cs.z + x[j + 1] * cs.w;
       }
       r0 = pack8(o);
       r1 = pack8(w);

@@ -30,7 +30,7 @@ using namespace tc5;
 
 constexpr int BC = 64;                  // rows per tile
 constexpr int STAGES = 3;
-constexpr uint32_t MIN_TILES = 2;       // tiles a CTA takes at least: fewer would spend more on the join than on the rows
+
 // How far (in powers of two) a score may exceed the reference m before m moves, and how far below the maximum m is then
 // put. Probabilities in f16 (beside four-bit rows) sit in its upper range, [2^7, 2^15] at the top, so that one of 2^-21 of
 // the largest is still a normal number; bf16 has the range of f32.
@@ -47,7 +47,7 @@ struct DecodeParams {
   float* part;                          // [2 * grid][heads_in][slot_rows][D + 4]: o, m, l
   uint32_t nq, heads, group, rows, row_tiles;   // rows = nq * group
   uint32_t slot_rows;                   // rows of a partial slot
-  uint32_t heads_in, min_tiles;         // NVFP4: KV heads of a CTA, tiles a CTA takes at least
+  uint32_t heads_in;                    // KV heads of a CTA (one over bf16 rows)
   uint32_t tile_rows;
   uint32_t box_rows;
   float scale_log2, cap_log2, inv_cap;          // cap_log2 = softcap * log2(e), inv_cap = scale / softcap
@@ -122,7 +122,7 @@ struct LinePlace {
   unsigned long long before;      // tiles before that sequence
 };
 // One warp: the line's length, and where tile `per * cta` of it lies.
-__device__ __forceinline__ LinePlace line_place(const PagedView& c, uint32_t nq, uint32_t tile, uint32_t items, uint32_t min_tiles,
+__device__ __forceinline__ LinePlace line_place(const PagedView& c, uint32_t nq, uint32_t tile, uint32_t items,
                                                 uint32_t grid, uint32_t cta, uint32_t lane) {
   LinePlace at;
   unsigned long long sum = 0;
@@ -131,7 +131,9 @@ __device__ __forceinline__ LinePlace line_place(const PagedView& c, uint32_t nq,
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
   at.total = sum;
-  at.per = max(min_tiles, uint32_t((sum + grid - 1) / grid));
+  // one tile is worth a CTA: with few tiles the chain of a CTA is what a call takes (777 rows of 8 heads: 9.0 us at one
+  // tile and up, 11.2 at two, 12.0 at four)
+  at.per = max(1u, uint32_t((sum + grid - 1) / grid));
   const unsigned long long want = (unsigned long long)at.per * cta;
   at.b = c.batch;
   at.before = 0;
@@ -198,7 +200,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   }
   mb_grid_dependency_sync();
   if (warp == 0) {
-    const LinePlace at = line_place(p.c, p.nq, BC, items, MIN_TILES, gridDim.x, blockIdx.x, lane);
+    const LinePlace at = line_place(p.c, p.nq, BC, items, gridDim.x, blockIdx.x, lane);
     if (lane == 0) {
       const unsigned long long first = (unsigned long long)at.per * blockIdx.x;
       place[0] = at.b;
@@ -489,6 +491,10 @@ paged_decode_kernel(const __grid_constant__ DecodeParams p) {
 // heads' scales of a row, are fetched once; the remaining factor of four goes along the rows. A step is 32 rows of one head:
 // packed bytes through a ring of the warp's own, both products with the codes expanded in registers. With four heads a
 // warp owns its head and nothing is joined inside the CTA.
+// Where row r of 16 V rows lies in shared memory: a lane reads rows 2 t4, which two 64-byte rows apart would all fall
+// into the same half of the banks; every second pair is swapped.
+__device__ __forceinline__ uint32_t v_place(uint32_t r) { return r ^ ((r >> 1) & 1u); }
+
 template <int D, int NT>
 struct DecodeFp4Shape {
   static constexpr int THREADS = 128;
@@ -496,8 +502,9 @@ struct DecodeFp4Shape {
   static constexpr int RAW16 = 2 * 16 * (D / 2) + 2 * 16 * (D / 16);           // 16 packed rows: K codes, V codes, K and V scales
   static constexpr int STAGES = 2;
   static constexpr int RING = 4 * STAGES * 2 * RAW16;
-  static constexpr int PATCH = 2 * NT * 8 * (D + 4) * 4 + 2 * 4 * NT * 8 * 4;  // two heads' o at most; m and l of the four warps
-  static constexpr int SMEM = RING + PATCH + 64;
+  static constexpr int PATCH = 2 * NT * 8 * (D + 4) * 4;                       // o of two heads at most, where warps share one
+  static constexpr int STATS = 2 * 4 * NT * 8 * 4;                             // m and l of the four warps
+  static constexpr int smem(bool joins) { return RING + STATS + 64 + (joins ? PATCH : 0); }
   static constexpr int CTAS = NT == 1 ? 4 : 3;
 };
 
@@ -507,10 +514,10 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
   using Shape = DecodeFp4Shape<D, NT>;
   constexpr int KS = D / 16, ROWS_Q = NT * 8, PD = D + 4, RAW16 = Shape::RAW16, STEP = 2 * RAW16;
   extern __shared__ __align__(128) uint8_t smem_fp4[];
-  float* patch = reinterpret_cast<float*>(smem_fp4 + Shape::RING);       // [heads_in][ROWS_Q][PD]
-  float* stat_m = patch + 2 * ROWS_Q * PD;                               // [warp][ROWS_Q]
+  float* stat_m = reinterpret_cast<float*>(smem_fp4 + Shape::RING);      // [warp][ROWS_Q]
   float* stat_l = stat_m + 4 * ROWS_Q;
   uint32_t* place = reinterpret_cast<uint32_t*>(stat_l + 4 * ROWS_Q);
+  float* patch = reinterpret_cast<float*>(place + 16);                   // [heads_in][ROWS_Q][PD], with fewer than four heads
   const int warp = __shfl_sync(0xFFFFFFFFu, int(threadIdx.x >> 5), 0);
   const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3u;
   const uint32_t hl = p.heads_in, rl = 4 / hl;                           // heads and row parts of the CTA
@@ -520,7 +527,7 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
 
   mb_grid_dependency_sync();
   if (warp == 0) {
-    const LinePlace at = line_place(p.c, p.nq, tile_rows, items, p.min_tiles, gridDim.x, blockIdx.x, lane);
+    const LinePlace at = line_place(p.c, p.nq, tile_rows, items, gridDim.x, blockIdx.x, lane);
     if (lane == 0) {
       const unsigned long long first = (unsigned long long)at.per * blockIdx.x;
       place[0] = at.b;
@@ -621,7 +628,7 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
             const bool in = int(c_row) + u * (32 / PER) < have;
             const size_t off = in ? c_off + size_t(u * (32 / PER)) * row_codes : 0;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + (lane + 32 * u) * 16u), "l"(pk + off), "r"(in ? 16u : 0u) : "memory");
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 16 * (D / 2) + (lane + 32 * u) * 16u), "l"(pv + off), "r"(in ? 16u : 0u) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + 16 * (D / 2) + (v_place(c_row + u * (32 / PER)) * PER + lane % PER) * 16u), "l"(pv + off), "r"(in ? 16u : 0u) : "memory");
           }
           const bool in = int(lane & 15u) < have;
           asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst + 16 * D + lane * (D / 16)),
@@ -650,14 +657,20 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
         // lane (g, t4): rows g and g + 8, features (D / 4) t4 .. of each
         uint32_t wlo[D / 32], whi[D / 32];
         __half2 sc[2][D / 64];                              // scales of the two rows, D / 64 blocks each
-#pragma unroll
-        for (int y = 0; y < D / 64; ++y) {
-          const uint2 a = *reinterpret_cast<const uint2*>(raw + g * (D / 2) + t4 * (D / 8) + 8 * y);
-          const uint2 c2 = *reinterpret_cast<const uint2*>(raw + (g + 8) * (D / 2) + t4 * (D / 8) + 8 * y);
-          wlo[2 * y] = a.x; wlo[2 * y + 1] = a.y;
-          whi[2 * y] = c2.x; whi[2 * y + 1] = c2.y;
-          sc[0][y] = __low2half2(e4m3x2_to_f16(raw[16 * D + g * (D / 16) + t4 * (D / 64) + y]));
-          sc[1][y] = __low2half2(e4m3x2_to_f16(raw[16 * D + (g + 8) * (D / 16) + t4 * (D / 64) + y]));
+        if (D == 128) {
+          const uint4 a = *reinterpret_cast<const uint4*>(raw + g * 64 + t4 * 16), c2 = *reinterpret_cast<const uint4*>(raw + (g + 8) * 64 + t4 * 16);
+          wlo[0] = a.x; wlo[1] = a.y; wlo[D / 32 - 2] = a.z; wlo[D / 32 - 1] = a.w;
+          whi[0] = c2.x; whi[1] = c2.y; whi[D / 32 - 2] = c2.z; whi[D / 32 - 1] = c2.w;
+          const __half2 s0 = e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(raw + 16 * D + g * 8 + t4 * 2));
+          const __half2 s1 = e4m3x2_to_f16(*reinterpret_cast<const uint16_t*>(raw + 16 * D + (g + 8) * 8 + t4 * 2));
+          sc[0][0] = __low2half2(s0); sc[0][D / 64 - 1] = __high2half2(s0);
+          sc[1][0] = __low2half2(s1); sc[1][D / 64 - 1] = __high2half2(s1);
+        } else {
+          const uint2 a = *reinterpret_cast<const uint2*>(raw + g * 32 + t4 * 8), c2 = *reinterpret_cast<const uint2*>(raw + (g + 8) * 32 + t4 * 8);
+          wlo[0] = a.x; wlo[1] = a.y;
+          whi[0] = c2.x; whi[1] = c2.y;
+          sc[0][0] = __low2half2(e4m3x2_to_f16(raw[16 * D + g * 4 + t4]));
+          sc[1][0] = __low2half2(e4m3x2_to_f16(raw[16 * D + (g + 8) * 4 + t4]));
         }
 #pragma unroll
         for (int w = 0; w < D / 32; ++w) {                  // a word of codes: two K steps
@@ -742,7 +755,7 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const uint32_t row = 2u * t4 + (q & 1u) + 8u * (q >> 1);
-          const uint32_t* src = reinterpret_cast<const uint32_t*>(vraw + row * (D / 2) + g * (D / 16));
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(vraw + v_place(row) * (D / 2) + g * (D / 16));
           if (W == 2) {
             const uint2 a = *reinterpret_cast<const uint2*>(src);
             w[q][0] = a.x; w[q][W - 1] = a.y;
@@ -931,11 +944,12 @@ paged_join_kernel(const __grid_constant__ DecodeParams p) {
 template <int D, bool FP4, int NT>
 int launch_decode(mb_ctx* ctx, cudaStream_t stream, const DecodeParams& p, uint32_t grid) {
   constexpr uint32_t once_bit = 1u << (4 * FP4 + 2 * (D == 128) + (NT - 1));
-  constexpr int smem = FP4 ? DecodeFp4Shape<D, NT>::SMEM : DecodeShape<D, NT>::SMEM;
+  constexpr int most = FP4 ? DecodeFp4Shape<D, NT>::smem(true) : DecodeShape<D, NT>::SMEM;
+  const int smem = FP4 ? DecodeFp4Shape<D, NT>::smem(p.heads_in < 4) : DecodeShape<D, NT>::SMEM;
   constexpr int threads = FP4 ? DecodeFp4Shape<D, NT>::THREADS : DecodeShape<D, NT>::THREADS;
   void (*kern)(DecodeParams) = FP4 ? paged_decode_fp4_kernel<D, NT> : paged_decode_kernel<D, NT>;
   if (!(ctx->paged_once.load(std::memory_order_acquire) & once_bit)) {
-    MB_CUDA_OK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    MB_CUDA_OK(ctx, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most));
     ctx->paged_once.fetch_or(once_bit, std::memory_order_release);
   }
   MB_CUDA_OK(ctx, mb_launch_pdl(kern, dim3(grid), dim3(threads), smem, stream, p));
@@ -993,7 +1007,6 @@ MB_API int mb_paged_decode(mb_ctx* ctx, mb_stream stream_, const void* q, size_t
   p.slot_rows = plan.slot_rows;
   p.heads_in = plan.heads_in;
   p.tile_rows = fp4 ? 32 * (4 / plan.heads_in) : uint32_t(BC);
-  p.min_tiles = 2 * plan.heads_in;            // 256 rows of a head
   p.meta = static_cast<uint4*>(workspace);
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan.meta_bytes);
   p.scale_log2 = terms->scale * 1.4426950408889634f;
