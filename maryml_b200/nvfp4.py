@@ -40,7 +40,8 @@ class PromptLane(enum.Enum):
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream of the current device (asked for without building a Stream object, which costs 3 us)."""
+    return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def _p(t):
