@@ -965,7 +965,12 @@ DecodePlan decode_plan(const mb_paged_kv* kv, size_t nq, size_t heads, int sms) 
   const bool fp4 = kv->elem == MB_KV_NVFP4, wide = rows > 8;
   r.row_tiles = uint32_t((rows + 15) / 16);
   r.slot_rows = wide ? 16 : 8;
-  r.heads_in = !fp4 ? 1 : kv->kv_heads % 4 == 0 ? 4 : kv->kv_heads % 2 == 0 ? 2 : 1;
+  // KV heads of a CTA over NVFP4 rows. Where the rows the call can reach stay in L2 together, a scale sector that four CTAs
+  // read comes from memory once all the same, and one head per CTA leaves a quarter of the pieces to join; beyond (half of
+  // L2: 60 MB of packed rows) four heads share it (8 KV heads of 128, four / one: 15.2 / 11.9 us at 1 x 2000 rows, 18.2 / 15.5
+  // at 4 x 4000, 111 / 188 at 32 x 13000).
+  const double reach = double(std::min(kv->pages, kv->batch * kv->table_width)) * double(kv->page_size) * double(kv->kv_heads * kv->d) * 1.125;
+  r.heads_in = !fp4 || reach <= 60.0e6 ? 1 : kv->kv_heads % 4 == 0 ? 4 : kv->kv_heads % 2 == 0 ? 2 : 1;
   r.grid = uint32_t(sms) * (fp4 ? (wide ? 3u : 4u) : 2u);
   r.meta_bytes = (kv->batch * kv->kv_heads / r.heads_in * r.row_tiles * sizeof(uint4) + 255) / 256 * 256;
   r.bytes = r.meta_bytes + size_t(r.grid) * 2 * r.heads_in * r.slot_rows * (kv->d + 4) * sizeof(float);

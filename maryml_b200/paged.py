@@ -181,7 +181,7 @@ def paged_append(qkv, cache, block_table, lens, inv_freq, cu_q=None, positions=N
 def paged_attention_decode(q, cache, block_table, lens, scale=None, softcap=0.0, window=0, slopes=None, prefix=None, out=None,
                            workspace=None):
     """Attention of the last nq tokens of every sequence: q [batch, nq, heads, head_dim] bf16 -> the same shape. Query i of
-    sequence b stands at position lens[b] - nq + i. scale: 1 / sqrt(head_dim) by default; softcap, window, slopes [heads]
+    sequence b stands at position lens[b] - nq + i; for blocks of eight tokens and more paged_attention_prompt is faster. scale: 1 / sqrt(head_dim) by default; softcap, window, slopes [heads]
     f32 and prefix [batch] int32 as in the header's mb_score_terms. A sequence of length 0 gets zeros. workspace: a buffer
     kept by the caller for calls that do not overlap; one is allocated otherwise."""
     _bf16(q, "q", cache.device)

@@ -184,6 +184,16 @@ def test_decode_terms(pg, terms, nvfp4):
     no_flags(pg)
 
 
+@pytest.mark.parametrize("terms", [{}, {"softcap": 30.0, "window": 333, "prefix": 130, "slopes": True}])
+@pytest.mark.parametrize("kvh,d,group,nq", [(4, 128, 4, 1), (8, 64, 2, 2), (2, 128, 8, 1), (6, 64, 3, 1), (4, 128, 12, 1)])
+def test_decode_nvfp4_heads_that_share_a_cta(pg, kvh, d, group, nq, terms):
+    """A pool larger than half of L2: four KV heads (two where four does not divide) of a CTA read the same rows."""
+    rows = int(62e6 / (kvh * d * 1.125))
+    s = Setup(pg, [3000, 64, 0, 129, 1, 777], 256, kvh, d, nvfp4=True, seed=kvh, spare=rows // 256 + 1, width=rows // 256 + 20)
+    run_decode(pg, s, kvh * group, nq, gain=3.0, **terms)
+    no_flags(pg)
+
+
 def test_decode_of_many_sequences_and_one_long_one(pg):
     """Lengths that differ by four orders of magnitude share the line of tiles; more than 32 sequences need the second
     round of the search for a CTA's first tile."""
@@ -685,7 +695,7 @@ def test_refusals(pg):
     cases = [
         lambda: dec(q=q.float()), lambda: dec(q=q[:, :, :, :64]), lambda: dec(q=q[:1]), lambda: dec(q=torch.zeros((2, 1, 7, 128), dtype=torch.bfloat16, device="cuda")),
         lambda: dec(t=s.table.long()), lambda: dec(t=s.table.t()), lambda: dec(t=s.table.cpu()), lambda: dec(n=s.lens[:1]), lambda: dec(n=s.lens.long()),
-        lambda: dec(scale=-1.0), lambda: dec(scale=float("nan")), lambda: dec(scale=0.0), lambda: dec(softcap=-1.0), lambda: dec(softcap=float("inf")),
+        lambda: dec(scale=-1.0), lambda: dec(scale=float("nan")), lambda: dec(scale=0.0), lambda: dec(softcap=-1.0), lambda: dec(softcap=float("inf")), lambda: dec(softcap=1e-40),
         lambda: dec(window=-3), lambda: dec(slopes=torch.zeros(7, device="cuda")), lambda: dec(slopes=torch.zeros(8, dtype=torch.float64, device="cuda")),
         lambda: dec(prefix=torch.zeros(3, dtype=torch.int32, device="cuda")), lambda: dec(prefix=torch.zeros(2, device="cuda")),
         lambda: dec(out=torch.zeros((2, 8, 128), dtype=torch.bfloat16, device="cuda")), lambda: dec(cache=bad_page),
