@@ -4,7 +4,9 @@
 // token once for all of its heads, and then walks the (token, head) units, d / 16 threads to a unit, a thread holding
 // the eight pairs (f, f + d / 2) of two 16-byte loads. Bound by HBM at prompt sizes (each value read once, written
 // once) and by the chain cu_q -> length -> table entry -> store at decode sizes; the loads of a thread's first unit
-// are issued before that chain.
+// are issued before that chain. Measured (32 query and 8 KV heads of 128): 3.0 us for one token, 3.4 us for 64, 37.9 us
+// for 8192 into bf16 pages (218 MB read and written, 0.88 of the copy rate), 21.4 us for 5095 into NVFP4 pages (110 MB,
+// 0.79; there the quantizer's instructions).
 #include "paged.cuh"
 #include "quant_block.cuh"
 

@@ -6,7 +6,10 @@
 // rescaled, only when a score exceeds it by a wide margin: no cross-lane maximum in the common tile.
 //
 // Bound by HBM for bf16 rows (each row of a sequence is read once, all query heads of a KV head ride along) and by
-// instruction issue for NVFP4 rows (the expansion of codes).
+// instruction issue for NVFP4 rows (the expansion of codes). Measured (32 query and 8 KV heads of 128): 165 us for 64
+// sequences of 1500 to 6700 bf16 rows (6.4 TB/s, 0.98 of the copy rate), 618 us for 32 of 32768 (6.9 TB/s), 9.0 us for one of
+// 777 (latency: two dependent launches); over NVFP4 rows 85 to 89 us for two tokens of 32 sequences, capped, with a window of
+// 8000 rows (298 MB, 0.53).
 //
 // Split. The lengths are known to the device only and differ from sequence to sequence, so the unit of work is one
 // 64-row tile of one (sequence, KV head, row tile) item; the tiles of all items form one line that is cut evenly over
