@@ -11,6 +11,7 @@ device, which must be the current device.
 """
 import ctypes as C
 import math
+import struct
 
 import torch
 
@@ -21,6 +22,9 @@ from ._lib import MaryError, lib, context
 # current stream is asked for without building a Stream object.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _bf16_t, _i32_t, _u8_t, _f32_t = torch.bfloat16, torch.int32, torch.uint8, torch.float32
+# mb_paged_kv and mb_score_terms as bytes (packing one costs a quarter of building the ctypes structure)
+_KV, _TERMS = struct.Struct("@PPPPiNNNNPNNPN"), struct.Struct("@ffNPP")
+assert _KV.size == C.sizeof(_lib.PagedKv) and _TERMS.size == C.sizeof(_lib.ScoreTerms)
 
 
 def _refuse(text):
@@ -30,12 +34,12 @@ def _refuse(text):
 def _int32(t, name, dims, dev):
     if t.dtype is not _i32_t or t.dim() != dims or t.device != dev:
         _refuse(f"{name} is a {dims}-d int32 tensor on {dev}, not {tuple(t.shape)} {t.dtype} on {t.device}")
-    if t.stride(dims - 1) != 1 and t.shape[-1] > 1:
+    if not t.is_contiguous() and t.stride(dims - 1) != 1:
         _refuse(f"{name} is read with unit stride in its last dimension, not {t.stride()}")
 
 
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return t.data_ptr() if t is not None else 0
 
 
 class PagedCache:
@@ -84,15 +88,16 @@ class PagedCache:
         return cls(make(2), make(2), make(16), make(16), head_dim)
 
     def _kv(self, block_table, lens):
+        """(sequences, mb_paged_kv as bytes)"""
         dev = self.device
         _int32(block_table, "block_table", 2, dev)
         _int32(lens, "lens", 1, dev)
         batch, width = block_table.shape
         if lens.shape[0] != batch:
             _refuse(f"block_table has {batch} rows, lens {lens.shape[0]} entries")
-        return _lib.PagedKv(self.k.data_ptr(), self.v.data_ptr(), _ptr(self.k_scales), _ptr(self.v_scales), self.elem, self.pages,
-                            self.page_size, self.kv_heads, self.head_dim, block_table.data_ptr(), width,
-                            block_table.stride(0) if batch > 1 else max(width, 1), lens.data_ptr(), batch)
+        return batch, _KV.pack(self.k.data_ptr(), self.v.data_ptr(), _ptr(self.k_scales), _ptr(self.v_scales), self.elem,
+                               self.pages, self.page_size, self.kv_heads, self.head_dim, block_table.data_ptr(), width,
+                               block_table.stride(0) if batch > 1 else max(width, 1), lens.data_ptr(), batch)
 
 
 def _terms(cache, batch, heads, scale, softcap, window, slopes, prefix):
@@ -105,8 +110,11 @@ def _terms(cache, batch, heads, scale, softcap, window, slopes, prefix):
             _refuse(f"prefix has {prefix.shape[0]} entries for {batch} sequences")
     if window < 0:
         _refuse(f"window is 0 (none) or a positive number of rows, not {window}")
-    return _lib.ScoreTerms(scale if scale is not None else 1.0 / math.sqrt(cache.head_dim), softcap, window, _ptr(slopes),
+    try:
+        return _TERMS.pack(scale if scale is not None else 1.0 / math.sqrt(cache.head_dim), softcap, window, _ptr(slopes),
                            _ptr(prefix))
+    except (struct.error, OverflowError, TypeError) as e:
+        _refuse(f"scale {scale}, softcap {softcap} and window {window} are two f32 numbers and a count: {e}")
 
 
 def _bf16(t, name, dev):
@@ -138,7 +146,7 @@ def paged_append(qkv, cache, block_table, lens, inv_freq, cu_q=None, positions=N
     (up to four axes) with `sections` = how many consecutive frequencies follow each axis. Returns the rotated queries
     [tokens, hq, head_dim]; rows at or past cu_q[batch] stay as they are in `out`."""
     dev, d = cache.device, cache.head_dim
-    kv = cache._kv(block_table, lens)
+    batch, kv = cache._kv(block_table, lens)
     if qkv.dtype is not _bf16_t or qkv.dim() != 2 or qkv.device != dev or qkv.stride(1) != 1:
         _refuse(f"qkv is a 2-d bf16 tensor on {dev} with unit stride along its rows")
     tokens, width = qkv.shape
@@ -149,8 +157,8 @@ def paged_append(qkv, cache, block_table, lens, inv_freq, cu_q=None, positions=N
         _refuse(f"inv_freq is {d // 2} contiguous f32 values on {dev}")
     if cu_q is not None:
         _int32(cu_q, "cu_q", 1, dev)
-        if cu_q.shape[0] != kv.batch + 1:
-            _refuse(f"cu_q has {cu_q.shape[0]} entries for {kv.batch} sequences")
+        if cu_q.shape[0] != batch + 1:
+            _refuse(f"cu_q has {cu_q.shape[0]} entries for {batch} sequences")
     axes, ends = 0, None
     if positions is not None:
         if positions.dim() == 1:
@@ -173,7 +181,7 @@ def paged_append(qkv, cache, block_table, lens, inv_freq, cu_q=None, positions=N
             _refuse(f"out is [{tokens}, {hq}, {d}], not {tuple(out.shape)}")
     ctx = context(dev.index)
     ctx.check(lib.mb_paged_append(ctx.handle, _raw_stream(dev.index), qkv.data_ptr(), qkv.stride(0) if tokens > 1 else width,
-                                  tokens, hq, C.byref(kv), _ptr(cu_q), inv_freq.data_ptr(), _ptr(positions), axes, ends,
+                                  tokens, hq, kv, _ptr(cu_q), inv_freq.data_ptr(), _ptr(positions), axes, ends,
                                   out.data_ptr()))
     return out
 
@@ -181,22 +189,23 @@ def paged_append(qkv, cache, block_table, lens, inv_freq, cu_q=None, positions=N
 def paged_attention_decode(q, cache, block_table, lens, scale=None, softcap=0.0, window=0, slopes=None, prefix=None, out=None,
                            workspace=None):
     """Attention of the last nq tokens of every sequence: q [batch, nq, heads, head_dim] bf16 -> the same shape. Query i of
-    sequence b stands at position lens[b] - nq + i; for blocks of eight tokens and more paged_attention_prompt is faster. scale: 1 / sqrt(head_dim) by default; softcap, window, slopes [heads]
-    f32 and prefix [batch] int32 as in the header's mb_score_terms. A sequence of length 0 gets zeros. workspace: a buffer
-    kept by the caller for calls that do not overlap; one is allocated otherwise."""
+    sequence b stands at position lens[b] - nq + i; for blocks of eight tokens and more paged_attention_prompt is faster.
+    scale: 1 / sqrt(head_dim) by default; softcap, window, slopes [heads] f32 and prefix [batch] int32 as in the header's
+    mb_score_terms. A sequence of length 0 gets zeros. workspace: a buffer kept by the caller for calls that do not overlap;
+    one is allocated otherwise."""
     _bf16(q, "q", cache.device)
     if q.dim() != 4 or q.shape[3] != cache.head_dim:
         _refuse(f"q is [batch, nq, heads, {cache.head_dim}], not {tuple(q.shape)}")
-    batch, nq, heads, _ = q.shape
-    kv = cache._kv(block_table, lens)
-    if batch != kv.batch:
-        _refuse(f"q has {batch} sequences, block_table {kv.batch}")
+    batch, kv = cache._kv(block_table, lens)
+    q_batch, nq, heads, _ = q.shape
+    if q_batch != batch:
+        _refuse(f"q has {q_batch} sequences, block_table {batch}")
     terms = _terms(cache, batch, heads, scale, softcap, window, slopes, prefix)
     out = _out_like(q, out)
     ctx = context(cache.device.index)
-    need = lib.mb_paged_decode_workspace(ctx.handle, C.byref(kv), nq, heads)
+    need = lib.mb_paged_decode_workspace(ctx.handle, kv, nq, heads)
     workspace = _workspace(workspace, need, cache.device)
-    ctx.check(lib.mb_paged_decode(ctx.handle, _raw_stream(ctx.device), q.data_ptr(), nq, heads, C.byref(kv), C.byref(terms),
+    ctx.check(lib.mb_paged_decode(ctx.handle, _raw_stream(ctx.device), q.data_ptr(), nq, heads, kv, terms,
                                   out.data_ptr(), _ptr(workspace), need))
     return out
 
@@ -211,15 +220,15 @@ def paged_attention_prompt(q, cu_q, cache, block_table, lens, scale=None, softca
     if q.dim() != 3 or q.shape[2] != cache.head_dim:
         _refuse(f"q is [tokens, heads, {cache.head_dim}], not {tuple(q.shape)}")
     tokens, heads, _ = q.shape
-    kv = cache._kv(block_table, lens)
+    batch, kv = cache._kv(block_table, lens)
     _int32(cu_q, "cu_q", 1, cache.device)
-    if cu_q.shape[0] != kv.batch + 1:
-        _refuse(f"cu_q has {cu_q.shape[0]} entries for {kv.batch} sequences")
-    terms = _terms(cache, kv.batch, heads, scale, softcap, window, slopes, prefix)
+    if cu_q.shape[0] != batch + 1:
+        _refuse(f"cu_q has {cu_q.shape[0]} entries for {batch} sequences")
+    terms = _terms(cache, batch, heads, scale, softcap, window, slopes, prefix)
     out = _out_like(q, out)
     ctx = context(cache.device.index)
-    need = lib.mb_paged_prompt_workspace(ctx.handle, C.byref(kv), tokens, heads)
+    need = lib.mb_paged_prompt_workspace(ctx.handle, kv, tokens, heads)
     workspace = _workspace(workspace, need, cache.device)
-    ctx.check(lib.mb_paged_prompt(ctx.handle, _raw_stream(ctx.device), q.data_ptr(), tokens, heads, C.byref(kv), cu_q.data_ptr(),
-                                  C.byref(terms), out.data_ptr(), _ptr(workspace) if need else None, need))
+    ctx.check(lib.mb_paged_prompt(ctx.handle, _raw_stream(ctx.device), q.data_ptr(), tokens, heads, kv, cu_q.data_ptr(),
+                                  terms, out.data_ptr(), _ptr(workspace) if need else None, need))
     return out

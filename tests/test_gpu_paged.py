@@ -695,7 +695,7 @@ def test_refusals(pg):
     cases = [
         lambda: dec(q=q.float()), lambda: dec(q=q[:, :, :, :64]), lambda: dec(q=q[:1]), lambda: dec(q=torch.zeros((2, 1, 7, 128), dtype=torch.bfloat16, device="cuda")),
         lambda: dec(t=s.table.long()), lambda: dec(t=s.table.t()), lambda: dec(t=s.table.cpu()), lambda: dec(n=s.lens[:1]), lambda: dec(n=s.lens.long()),
-        lambda: dec(scale=-1.0), lambda: dec(scale=float("nan")), lambda: dec(scale=0.0), lambda: dec(softcap=-1.0), lambda: dec(softcap=float("inf")), lambda: dec(softcap=1e-40),
+        lambda: dec(scale=-1.0), lambda: dec(scale=float("nan")), lambda: dec(scale=0.0), lambda: dec(softcap=-1.0), lambda: dec(softcap=float("inf")), lambda: dec(softcap=1e-40), lambda: dec(softcap=1e40), lambda: dec(window=1 << 70), lambda: dec(window=1.5),
         lambda: dec(window=-3), lambda: dec(slopes=torch.zeros(7, device="cuda")), lambda: dec(slopes=torch.zeros(8, dtype=torch.float64, device="cuda")),
         lambda: dec(prefix=torch.zeros(3, dtype=torch.int32, device="cuda")), lambda: dec(prefix=torch.zeros(2, device="cuda")),
         lambda: dec(out=torch.zeros((2, 8, 128), dtype=torch.bfloat16, device="cuda")), lambda: dec(cache=bad_page),
