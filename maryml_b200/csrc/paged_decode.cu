@@ -7,9 +7,9 @@
 //
 // Bound by HBM for bf16 rows (each row of a sequence is read once, all query heads of a KV head ride along) and by
 // instruction issue for NVFP4 rows (the expansion of codes). Measured (32 query and 8 KV heads of 128): 165 us for 64
-// sequences of 1500 to 6700 bf16 rows (6.4 TB/s, 0.98 of the copy rate), 618 us for 32 of 32768 (6.9 TB/s), 9.0 us for one of
-// 777 (latency: two dependent launches); over NVFP4 rows 85 to 89 us for two tokens of 32 sequences, capped, with a window of
-// 8000 rows (298 MB, 0.53).
+// sequences of 1500 to 6700 bf16 rows (6.4 TB/s, 0.98 of the copy rate), 618 us for 32 of 32768 (6.9 TB/s), 8.0 us for one of
+// 777 (latency: two dependent launches); over NVFP4 rows 83 to 85 us for two tokens of 32 sequences, capped, with a window of
+// 8000 rows (298 MB, 0.54).
 //
 // Split. The lengths are known to the device only and differ from sequence to sequence, so the unit of work is one
 // 64-row tile of one (sequence, KV head, row tile) item; the tiles of all items form one line that is cut evenly over
@@ -462,7 +462,7 @@ paged_decode_kernel(const __grid_constant__ DecodeParams p) {
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float mw = stat_m[w * ROWS + r];
-          ll += mw == -INFINITY ? 0.0f : stat_l[w * ROWS + r] * paged_ex2(mw - mm);
+          ll += mw == -INFINITY ? stat_l[w * ROWS + r] : stat_l[w * ROWS + r] * paged_ex2(mw - mm);   // without a score: 0, or NaN
         }
         const float4 v = *reinterpret_cast<const float4*>(patch + r * PD + d4);
         if (complete) {
@@ -824,7 +824,7 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
           for (uint32_t w = head_in; w < 4; w += hl) mm = fmaxf(mm, stat_m[w * ROWS_Q + r]);
           for (uint32_t w = head_in; w < 4; w += hl) {
             const float mw = stat_m[w * ROWS_Q + r];
-            ll += mw == -INFINITY ? 0.0f : stat_l[w * ROWS_Q + r] * paged_ex2(mw - mm);
+            ll += mw == -INFINITY ? stat_l[w * ROWS_Q + r] : stat_l[w * ROWS_Q + r] * paged_ex2(mw - mm);   // without a score: 0, or NaN
           }
           const float f = m[nt][e] == -INFINITY ? 0.0f : paged_ex2(m[nt][e] - mm);
 #pragma unroll
@@ -893,7 +893,9 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
   }
 }
 
-// out = sum over pieces, in tile order. One block per query row: groups of D / 4 threads (four values each) walk the pieces.
+// out = sum over pieces, in an order of their own. One block per query row: groups of D / 4 threads (four values each) walk
+// the pieces. Bound by the chain of its loads; with the item's place asked for before the length and the first pieces'
+// values before their references are compared, a call over 777 rows takes 8.0 instead of 9.0 us.
 template <int D>
 __global__ void __launch_bounds__(128)
 paged_join_kernel(const __grid_constant__ DecodeParams p) {
@@ -904,6 +906,8 @@ paged_join_kernel(const __grid_constant__ DecodeParams p) {
   const uint32_t h = blockIdx.x % p.heads, qi = (blockIdx.x / p.heads) % p.nq, b = blockIdx.x / (p.heads * p.nq);
   const uint32_t kvh = h / p.group, r = qi * p.group + (h - kvh * p.group), items = p.c.kv_heads / p.heads_in * p.row_tiles;
   int len;
+  // asked for before the length is known: the chain of loads is what the join takes (an item without tiles has none written)
+  const uint4 meta = __ldcg(p.meta + size_t(b) * items + kvh / p.heads_in * p.row_tiles + r / 16);
   const PagedSpan span = decode_span(p.c, b, p.nq, p.tile_rows, len);
   __nv_bfloat16* dst = p.out + size_t(blockIdx.x) * D;
   if (threadIdx.x == 0 && paged_len_bad(p.c, b)) paged_raise(p.c, b);
@@ -911,27 +915,43 @@ paged_join_kernel(const __grid_constant__ DecodeParams p) {
     for (uint32_t d = threadIdx.x; d < D; d += 128) dst[d] = __float2bfloat16_rn(0.0f);
     return;
   }
-  const uint4 meta = p.meta[size_t(b) * items + kvh / p.heads_in * p.row_tiles + r / 16];
   const uint32_t pieces = meta.y;
   if (pieces == 1) return;
   const float* row = p.part + size_t(r % 16) * (D + 4);
   auto slot_of = [&](uint32_t i) {
     return (size_t(2 * (meta.z + i) + (i == 0 ? meta.x : 0u)) * p.heads_in + kvh % p.heads_in) * p.slot_rows * (D + 4);
   };
+  const uint32_t lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  // the first pieces' values are on their way while the references are compared
+  constexpr int AHEAD = 4;
+  float4 v[AHEAD];
+  float mw[AHEAD], lw[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const uint32_t i = grp + k * GROUPS;
+    const float* src = row + slot_of(min(i, pieces - 1));
+    v[k] = *reinterpret_cast<const float4*>(src + lane * 4);
+    mw[k] = i < pieces ? src[D] : -INFINITY;
+    lw[k] = i < pieces ? src[D + 1] : 0.0f;
+  }
   float mm = -INFINITY;
   for (uint32_t i = threadIdx.x & 31; i < pieces; i += 32) mm = fmaxf(mm, row[slot_of(i) + D]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xFFFFFFFFu, mm, o));
-  const uint32_t lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   float ll = 0.0f;
+  auto add = [&](const float4& x, float m, float l) {
+    if (m == -INFINITY) { ll += l; return; }              // nothing seen there (0), or NaN alone
+    const float f = exp2f(m - mm);
+    acc.x = fmaf(x.x, f, acc.x); acc.y = fmaf(x.y, f, acc.y); acc.z = fmaf(x.z, f, acc.z); acc.w = fmaf(x.w, f, acc.w);
+    ll = fmaf(l, f, ll);
+  };
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) add(v[k], mw[k], lw[k]);
 #pragma unroll 4
-  for (uint32_t i = grp; i < pieces; i += GROUPS) {
+  for (uint32_t i = grp + AHEAD * GROUPS; i < pieces; i += GROUPS) {
     const float* src = row + slot_of(i);
-    const float mw = src[D], f = mw == -INFINITY ? 0.0f : exp2f(mw - mm);
-    const float4 v = *reinterpret_cast<const float4*>(src + lane * 4);
-    acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
-    ll = fmaf(src[D + 1], f, ll);
+    add(*reinterpret_cast<const float4*>(src + lane * 4), src[D], src[D + 1]);
   }
   *reinterpret_cast<float4*>(&acc_s[grp][lane * 4]) = acc;
   if (lane == 0) l_s[grp] = ll;

@@ -671,6 +671,23 @@ def test_masked_keys_may_hold_anything(pg):
     no_flags(pg)
 
 
+def test_nan_in_a_key_that_is_seen_comes_out(pg):
+    """A NaN in a row of K makes the rows that see it NaN, alone or among others, in one piece or joined, and no other row."""
+    for d in (64, 128):
+        for softcap in (0.0, 20.0):
+            s = Setup(pg, [40, 1, 2000, 7], 32, 2, d, seed=62)
+            row = lambda b, r: int(s.table[b, r // 32]) * 32 + r % 32
+            k = s.cache.k.view(-1, 2, d)
+            for b, r in ((0, 17), (1, 0), (2, 1234)):
+                k[row(b, r), 0, 3] = float("nan")                 # the first KV head only
+            q = torch.randn((4, 1, 8, d), device="cuda", generator=s.gen).to(torch.bfloat16)
+            cu = torch.arange(5, dtype=torch.int32, device="cuda")
+            for out in (pg.paged_attention_decode(q, s.cache, s.table, s.lens, softcap=softcap).view(4, 8, d),
+                        pg.paged_attention_prompt(q.view(4, 8, d), cu, s.cache, s.table, s.lens, softcap=softcap)):
+                assert out[:3, :4].isnan().all() and out[3].isfinite().all() and out[:, 4:].isfinite().all()
+    no_flags(pg)
+
+
 def test_zero_tokens_are_a_call_that_does_nothing(pg):
     s = Setup(pg, [5, 6], 16, 2, 128, seed=61)
     cu = torch.zeros(3, dtype=torch.int32, device="cuda")
