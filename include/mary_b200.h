@@ -487,8 +487,8 @@ typedef struct mb_paged_kv {
 } mb_paged_kv;
 
 /* What happens to a score s = scale * q.k of the query at position p and the key at position k:
- * s' = softcap * tanh(s / softcap) when softcap > 0, then s' - slopes[head] * |p - k| when slopes is given
- * ([heads] f32). The key is visible when k <= p and, with window > 0, p - k < window; keys k < prefix[b]
+ * s' = softcap * tanh(s / softcap) when softcap > 0 (scale and softcap are at most 1e18), then s' - slopes[head] * |p - k|
+ * when slopes is given ([heads] f32). The key is visible when k <= p and, with window > 0, p - k < window; keys k < prefix[b]
  * (prefix [batch] i32 or NULL) are visible to every query of sequence b, later ones included: a two-way prefix, or,
  * beside a window, first rows that stay in sight. A query that sees no key gets a row of zeros. */
 typedef struct mb_score_terms {

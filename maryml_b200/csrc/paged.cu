@@ -271,8 +271,9 @@ int paged_view(mb_ctx* ctx, const char* what, const mb_paged_kv* kv, const mb_sc
     MB_REQUIRE(ctx, kv->k_scales && kv->v_scales && mb_aligned(kv->k_scales, 8) && mb_aligned(kv->v_scales, 8),
                "%s: NVFP4 pools need 8-byte aligned scales", what);
   if (terms) {
-    MB_REQUIRE(ctx, terms->scale > 0.0f && terms->scale <= 3.0e38f, "%s: scale must be positive and finite", what);
-    MB_REQUIRE(ctx, terms->softcap >= 0.0f && terms->softcap <= 3.0e38f, "%s: softcap must be zero (none) or positive and finite", what);
+    MB_REQUIRE(ctx, terms->scale > 0.0f && terms->scale <= 1.0e18f, "%s: scale must be positive and at most 1e18", what);
+    MB_REQUIRE(ctx, terms->softcap >= 0.0f && terms->softcap <= 1.0e18f, "%s: softcap must be zero (none) or positive and at most 1e18",
+               what);
     MB_REQUIRE(ctx, terms->softcap == 0.0f || terms->scale / terms->softcap <= 3.0e38f, "%s: softcap %g is too small for the scale", what,
                double(terms->softcap));
     MB_REQUIRE(ctx, mb_aligned(terms->slopes, 4) && mb_aligned(terms->prefix, 4), "%s: slopes and prefix need 4-byte alignment", what);

@@ -96,12 +96,24 @@ __device__ __forceinline__ float paged_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// tanh(x) with an absolute error of a few 2^-24 for every x: 1 - 2 / (e^2x + 1), saturating at +-1 through e^2x = inf
-// or 0. An absolute error is what a capped score needs (it is multiplied by the cap and added to an exponent);
-// the one-instruction tanh is off by 2^-11 of its value, 0.02 in a score near a cap of 50.
-__device__ __forceinline__ float paged_tanh(float x) {
+// tanh(x) of a score over its cap: 1 - 2 / (e^2x + 1), saturating at +-1 through e^2x = inf or 0, with an absolute error of a
+// few 2^-24. The cap multiplies that error into an exponent of two: up to cap * log2(e) = 512 it stays below 2e-4, an eighth
+// of the rounding of a bf16 probability. A larger cap may be any number of times the score, so there values below 1/2 are
+// x + x^3 q(x^2), q of degree two (a weighted least-squares fit, reweighted towards the smallest maximum; off by 1.9e-7
+// and by 1.0e-6 of its value at most). The one-instruction tanh is off by 2^-11 of its value, 0.02 in a score near a cap of
+// 50. The decode kernels choose by the cap (83.5 us against 86.1 with the second form always, two tokens of 32 sequences over
+// four-bit rows); the general form of the prompt kernel always takes both (263 us against 270 by the cap, 2 x 515 tokens
+// over 12000 rows).
+constexpr float PAGED_LARGE_CAP = 512.0f;
+__device__ __forceinline__ float paged_tanh(float x, bool large_cap) {
   const float e = paged_ex2(x * 2.8853900817779268f);    // 2 log2(e)
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(e + 1.0f));
-  return fmaf(-2.0f, r, 1.0f);
+  r = fmaf(-2.0f, r, 1.0f);
+  if (large_cap) {
+    const float y = x * x;
+    const float q = fmaf(fmaf(-4.422929382e-02f, y, 1.318586219e-01f), y, -3.332646081e-01f);
+    r = fabsf(x) < 0.5f ? fmaf(x * y, q, x) : r;
+  }
+  return r;
 }

@@ -8,7 +8,7 @@
 // Bound by HBM for bf16 rows (each row of a sequence is read once, all query heads of a KV head ride along) and by
 // instruction issue for NVFP4 rows (the expansion of codes). Measured (32 query and 8 KV heads of 128): 165 us for 64
 // sequences of 1500 to 6700 bf16 rows (6.4 TB/s, 0.98 of the copy rate), 618 us for 32 of 32768 (6.9 TB/s), 8.0 us for one of
-// 777 (latency: two dependent launches); over NVFP4 rows 83 to 85 us for two tokens of 32 sequences, capped, with a window of
+// 777 (latency: two dependent launches); over NVFP4 rows 83 to 86 us for two tokens of 32 sequences, capped, with a window of
 // 8000 rows (298 MB, 0.54).
 //
 // Split. The lengths are known to the device only and differ from sequence to sequence, so the unit of work is one
@@ -342,7 +342,8 @@ paged_decode_kernel(const __grid_constant__ DecodeParams p) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int key = row0 + int(g) + (e >= 2 ? 8 : 0), qp = qpos[nt][e & 1];
-            float y = p.cap_log2 > 0.0f ? p.cap_log2 * paged_tanh(s[nt][e] * p.inv_cap) : s[nt][e] * p.scale_log2;
+            float y = p.cap_log2 > 0.0f ? p.cap_log2 * paged_tanh(s[nt][e] * p.inv_cap, p.cap_log2 > PAGED_LARGE_CAP)
+                                        : s[nt][e] * p.scale_log2;
             if (p.slopes) y = fmaf(-slope[nt][e & 1], fabsf(float(qp - key)), y);
             if (!whole) {
               const bool seen = (key < len && key <= qp && (p.c.window == 0 || qp - key < int(p.c.window))) || key < span.prefix;
@@ -692,7 +693,8 @@ paged_decode_fp4_kernel(const __grid_constant__ DecodeParams p) {
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            float y = p.cap_log2 > 0.0f ? p.cap_log2 * paged_tanh(s[nt][e] * p.inv_cap) : s[nt][e] * p.scale_log2;
+            float y = p.cap_log2 > 0.0f ? p.cap_log2 * paged_tanh(s[nt][e] * p.inv_cap, p.cap_log2 > PAGED_LARGE_CAP)
+                                        : s[nt][e] * p.scale_log2;
             if (p.slopes) y = fmaf(-slope[nt][e & 1], fabsf(float(qpos[nt][e & 1] - (row0 + 16 * h + int(g) + (e >= 2 ? 8 : 0)))), y);
             x[h][nt][e] = y;
           }

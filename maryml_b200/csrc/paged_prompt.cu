@@ -20,8 +20,8 @@
 // special-function unit), PV (512), and the hand-offs between them; two query tiles alternate, and TMEM (two score tiles and
 // two outputs, 4 x 128 columns at D = 128) has no room for a third. Cycle counters at 8192 tokens: 3624 per key tile of both
 // query tiles, of which the tensor pipe works 2048 and a group waits 1110 for its scores. Measured (32 query and 8 KV heads
-// of 128): 462 us for 8192 tokens (1190 TFLOP/s of the pairs under the mask, 0.72 of the measured burst), 272 us for 2 x 515
-// tokens over 12000 rows, capped (782 TFLOP/s), 111 us for 3 x 1600 tokens over NVFP4 pages with bias and prefix.
+// of 128): 462 us for 8192 tokens (1190 TFLOP/s of the pairs under the mask, 0.72 of the measured burst), 263 to 283 us for
+// 2 x 515 tokens over 12000 rows, capped (751 to 808 TFLOP/s, by the machine), 111 us for 3 x 1600 tokens over NVFP4 pages with bias and prefix.
 //
 // Roles: warp 0 loads (TMA; boxes never cross a page), warp 1 issues, warps 4-7 and 8-11 are the softmax groups, a thread
 // per row. Over NVFP4 pages warps 0, 2, 3 and 12 expand rows to bf16 into the same swizzled tiles (exact: code x scale has
@@ -99,8 +99,11 @@ __device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) {
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// tanh of two values with |x| <= 1: x + x^3 q(x^2), q of degree four, off by 3.3e-7 at most (a weighted
-// least-squares fit, reweighted towards the smallest maximum). As exact as paged_tanh in the absolute error that counts, and without its two special-function operations.
+// tanh of two values with |x| <= 1: x + x^3 q(x^2), q of degree four, off by 3.3e-7 and by 1.3e-6 of its value at most (a
+// weighted least-squares fit, reweighted towards the smallest maximum). Without the two special-function operations of
+// paged_tanh. The powers of c moved into the coefficients save an operation a pair and no time (263 us either way at 2 x 515
+// tokens over 12000 rows); a shorter fit for units within half the cap, five operations instead of eight, costs registers
+// and its second copy of the pass more than it saves (270 us).
 __device__ __forceinline__ f32x2 tanh_pair(f32x2 x) {
   const f32x2 y = f2_mul(x, x);
   f32x2 q = f2_fma(f2_pack(-2.983081579e-03f, -2.983081579e-03f), y, f2_pack(1.653281572e-02f, 1.653281572e-02f));
@@ -582,7 +585,7 @@ paged_prompt_kernel(const __grid_constant__ PromptParams p) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               float y = __uint_as_float(sr[i]);
-              y = (CAPPED ? paged_tanh(y * p.inv_cap) : y) * mult;
+              y = (CAPPED ? paged_tanh(y * p.inv_cap, true) : y) * mult;
               if (BIASED) y = fmaf(-slope, fabsf(away - float(i)), y);
               x[i] = seen & (1u << i) ? y : -INFINITY;
             }

@@ -276,6 +276,28 @@ def test_prompt_terms(pg, terms, nvfp4):
     no_flags(pg)
 
 
+@pytest.mark.parametrize("gain,softcap", [(1.0, 50.0), (4.0, 50.0), (4.0, 12.0), (16.0, 20.0), (4.0, 1e-6), (4.0, 1e-3),
+                                          (4.0, 355.0), (64.0, 355.0), (4.0, 1e4), (4.0, 1e8), (4.0, 1e18)])
+def test_caps_of_every_size(pg, gain, softcap):
+    """Scores far below the cap (where only the relative error of the tanh helps), near it and far beyond."""
+    for d, heads in ((128, 4), (64, 2)):
+        run_prompt(pg, Setup(pg, [700], 64, 1, d, seed=d + 1), heads, [300], gain=gain, softcap=softcap)
+        run_decode(pg, Setup(pg, [700, 3], 64, 1, d, seed=d + 1), heads, 1, gain=gain, softcap=softcap)
+    no_flags(pg)
+
+
+def test_scales_and_caps_that_leave_f32_are_refused(pg):
+    from maryml_b200 import MaryError
+    s = Setup(pg, [20, 30], 16, 2, 128, seed=71)
+    q, cu = torch.zeros((2, 1, 8, 128), dtype=torch.bfloat16, device="cuda"), torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for terms in ({"softcap": 3e38}, {"softcap": 1e19}, {"scale": 3e38}, {"scale": 1e19}):
+        with pytest.raises(MaryError):
+            pg.paged_attention_decode(q, s.cache, s.table, s.lens, **terms)
+        with pytest.raises(MaryError):
+            pg.paged_attention_prompt(q[:, 0], cu, s.cache, s.table, s.lens, **terms)
+    no_flags(pg)
+
+
 def test_prompt_scores_that_outgrow_their_reference(pg):
     """Keys whose scores rise by more than 2^40 towards the sequence's start, the last tiles to be read: every tile moves
     the running reference and rescales the output. The queries and keys are such that scores are exact."""
